@@ -1,0 +1,241 @@
+// Rows of the cache moved inside their own tensors: pages copied to other pages, and the states of a request's beams passed on to the beams that
+// come of them.  Nothing is computed: what bounds both is reading every row that is copied once and writing every row that is overwritten once.
+//
+// A tensor is [outer, rows, ...] with the bytes of a row in one piece; "row r" is the rows r of all its outer entries (a page of every layer, the
+// state of a request in every layer).  Sizes, strides and starts may be any: 16 bytes go at a time where all of them allow it, else 8, 4, 2 or 1.
+#include "common.cuh"
+
+#define ROWS_TENSORS 16                                         // tensors of one launch
+#define ROWS_THREADS 256
+#define ROWS_LOADS 4                                            // loads of a thread under way
+#define ROWS_SPAN (ROWS_THREADS * ROWS_LOADS)                   // units of a block
+#define ROWS_BEAMS 32                                           // places of a group: lanes of a warp
+
+__device__ int g_rows_status = 0;    // 0 = fine; 1 = an index outside a tensor was passed over
+// Reads the word and sets it back.
+PICO_API int pico_rows_status(int* out) {
+    const cudaError_t e = cudaMemcpyFromSymbol(out, g_rows_status, sizeof(int), 0, cudaMemcpyDeviceToHost);
+    const int fine = 0;
+    return (int)(e == cudaSuccess && *out ? cudaMemcpyToSymbol(g_rows_status, &fine, sizeof(int), 0, cudaMemcpyHostToDevice) : e);
+}
+
+struct RowTensor {
+    char* base;
+    long long outer_stride, row_stride;  // bytes
+    unsigned units, total;               // of a row; of a row in all outer entries
+    int rows, unit;                      // unit: bytes
+    int first;                           // the first block (x) that works on this tensor
+};
+struct RowTensors {
+    RowTensor t[ROWS_TENSORS];
+    int n;
+};
+
+// The place of unit i of row 0.
+__device__ __forceinline__ long long row_unit(const RowTensor& t, unsigned i) {
+    const unsigned o = i / t.units;
+    return (long long)o * t.outer_stride + (long long)(i - o * t.units) * t.unit;
+}
+__device__ __forceinline__ int rows_tensor(const RowTensors& ts, int block) {
+    int k = 0;
+    while (k + 1 < ts.n && block >= ts.t[k + 1].first) ++k;
+    return k;
+}
+
+template <typename U>
+__device__ __forceinline__ void copy_units(const RowTensor& t, int block, int src, int dst) {
+    const long long from = (long long)src * t.row_stride, to = (long long)dst * t.row_stride;
+    const unsigned i0 = (unsigned)block * ROWS_SPAN + threadIdx.x;
+    U v[ROWS_LOADS];
+    long long at[ROWS_LOADS];
+#pragma unroll
+    for (int u = 0; u < ROWS_LOADS; ++u) {
+        const unsigned i = i0 + u * ROWS_THREADS;
+        if (i < t.total) {
+            at[u] = row_unit(t, i);
+            v[u] = *reinterpret_cast<const U*>(t.base + at[u] + from);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS_LOADS; ++u)
+        if (i0 + u * ROWS_THREADS < t.total) *reinterpret_cast<U*>(t.base + at[u] + to) = v[u];
+}
+
+// Grid (blocks of a row over all tensors, pairs): row dst[y] becomes row src[y].  A pair with a negative index, or of a row with itself, is passed over.
+__global__ void __launch_bounds__(ROWS_THREADS) copy_rows_kernel(RowTensors ts, const int* __restrict__ src, const int* __restrict__ dst) {
+    pdl_launch_dependents();
+    const RowTensor t = ts.t[rows_tensor(ts, blockIdx.x)];
+    pdl_wait();
+    const int s = src[blockIdx.y], d = dst[blockIdx.y];
+    if (s < 0 || d < 0 || s == d) return;
+    if (s >= t.rows || d >= t.rows) {
+        if (threadIdx.x == 0) g_rows_status = 1;
+        return;
+    }
+    const int block = blockIdx.x - t.first;
+    if (t.unit == 16) copy_units<uint4>(t, block, s, d);
+    else if (t.unit == 8) copy_units<uint2>(t, block, s, d);
+    else if (t.unit == 4) copy_units<unsigned>(t, block, s, d);
+    else if (t.unit == 2) copy_units<unsigned short>(t, block, s, d);
+    else copy_units<unsigned char>(t, block, s, d);
+}
+
+// What a group's block has to do, in order: row to[i] becomes row from[i].  from -1: the row that was put aside; to -1: puts the row aside.
+struct RowMoves {
+    int n;
+    int from[2 * ROWS_BEAMS], to[2 * ROWS_BEAMS];
+};
+
+template <typename U>
+__device__ __forceinline__ void move_units(const RowTensor& t, int block, const RowMoves& m) {
+    const unsigned i0 = (unsigned)block * ROWS_SPAN + threadIdx.x;
+    char* at[ROWS_LOADS];
+    bool in[ROWS_LOADS];
+    U aside[ROWS_LOADS];
+#pragma unroll
+    for (int u = 0; u < ROWS_LOADS; ++u) {
+        const unsigned i = i0 + u * ROWS_THREADS;
+        in[u] = i < t.total;
+        at[u] = t.base + (in[u] ? row_unit(t, i) : 0);
+        aside[u] = U();
+    }
+    // four moves at a time, loads first: a row is overwritten only after the moves before it have read it
+    for (int k0 = 0; k0 < m.n; k0 += 4) {
+        U v[4][ROWS_LOADS];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k0 + k < m.n && m.from[k0 + k] >= 0) {
+                const long long from = (long long)m.from[k0 + k] * t.row_stride;
+#pragma unroll
+                for (int u = 0; u < ROWS_LOADS; ++u)
+                    if (in[u]) v[k][u] = *reinterpret_cast<const U*>(at[u] + from);
+            }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k0 + k < m.n) {
+                if (m.to[k0 + k] < 0) {
+#pragma unroll
+                    for (int u = 0; u < ROWS_LOADS; ++u) aside[u] = v[k][u];
+                } else {
+                    const long long to = (long long)m.to[k0 + k] * t.row_stride;
+#pragma unroll
+                    for (int u = 0; u < ROWS_LOADS; ++u)
+                        if (in[u]) *reinterpret_cast<U*>(at[u] + to) = m.from[k0 + k] >= 0 ? v[k][u] : aside[u];
+                }
+            }
+    }
+}
+
+// Grid (blocks of a row over all tensors, groups): rows slots[g, p] become what rows slots[g, parents[g, p]] were, at once.  Every byte of a group's rows
+// is read and written by one thread, in an order in which a row is overwritten after all that read it have; one row of a cycle is put aside.
+__global__ void __launch_bounds__(ROWS_THREADS) reorder_rows_kernel(RowTensors ts, const int* __restrict__ slots, const int* __restrict__ parents, int places) {
+    pdl_launch_dependents();
+    __shared__ RowMoves moves;
+    __shared__ unsigned readers[ROWS_BEAMS];
+    const RowTensor t = ts.t[rows_tensor(ts, blockIdx.x)];
+    pdl_wait();
+    if (threadIdx.x < 32) {
+        const int p = threadIdx.x;
+        const int slot = p < places ? slots[blockIdx.y * places + p] : -1, parent = p < places ? parents[blockIdx.y * places + p] : p;
+        int from = __shfl_sync(0xffffffffu, slot, parent & 31);
+        bool wanted = p < places && parent != p;
+        if (wanted && (parent < 0 || parent >= places || slot < 0 || slot >= t.rows || from < 0 || from >= t.rows)) {
+            g_rows_status = 1;
+            wanted = false;
+        }
+        // the places that wait to take over what place p holds
+        readers[p] = 0u;
+        __syncwarp();
+        const unsigned same = __match_any_sync(0xffffffffu, wanted ? parent : 32 + p);
+        if (wanted) readers[parent] = same;
+        __syncwarp();
+        unsigned waiting = readers[p];
+        unsigned todo = __ballot_sync(0xffffffffu, wanted);
+        int n = 0;
+        while (todo) {
+            const unsigned ready = __ballot_sync(0xffffffffu, ((todo >> p) & 1u) && !(waiting & todo));
+            if (ready) {
+                if ((ready >> p) & 1u) {
+                    const int at = n + __popc(ready & ((1u << p) - 1u));
+                    moves.from[at] = from;
+                    moves.to[at] = slot;
+                }
+                n += __popc(ready);
+                todo &= ~ready;
+            } else {
+                // cycles are left, in which every place is read once: what the first holds is put aside for its reader, which is done before
+                // another row is put aside
+                const int aside = __ffs(todo) - 1;
+                if (p == aside) {
+                    moves.from[n] = slot;
+                    moves.to[n] = -1;
+                    waiting = 0u;
+                }
+                if (((todo >> p) & 1u) && parent == aside) from = -1;
+                ++n;
+            }
+        }
+        if (p == 0) moves.n = n;
+    }
+    __syncthreads();
+    if (moves.n == 0) return;
+    const int block = blockIdx.x - t.first;
+    if (t.unit == 16) move_units<uint4>(t, block, moves);
+    else if (t.unit == 8) move_units<uint2>(t, block, moves);
+    else if (t.unit == 4) move_units<unsigned>(t, block, moves);
+    else if (t.unit == 2) move_units<unsigned short>(t, block, moves);
+    else move_units<unsigned char>(t, block, moves);
+}
+
+// What a launch needs to know of n tensors.  of: six numbers for each - address, outer entries, rows, bytes between outer entries, bytes between rows, bytes
+// of a row.  Returns the blocks (x) of the launch, or a negative code.
+static long long rows_describe(const long long* of, int n, RowTensors& ts) {
+    ts.n = 0;
+    long long blocks = 0;
+    for (int i = 0; i < n; ++i) {
+        const long long base = of[6 * i], outer = of[6 * i + 1], rows = of[6 * i + 2], outer_stride = of[6 * i + 3], row_stride = of[6 * i + 4], bytes = of[6 * i + 5];
+        if (outer < 1 || rows < 1 || bytes < 1) continue;
+        if (rows > 0x7fffffffll || outer_stride < 0 || row_stride < 0) return PICO_ERR_SIZE;
+        const long long all = base | bytes | (outer > 1 ? outer_stride : 0) | (rows > 1 ? row_stride : 0);
+        const int unit = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
+        if (bytes / unit > 0x7fffffffll / outer) return PICO_ERR_SIZE;
+        RowTensor& t = ts.t[ts.n++];
+        t.base = reinterpret_cast<char*>(base);
+        t.outer_stride = outer_stride;
+        t.row_stride = row_stride;
+        t.units = (unsigned)(bytes / unit);
+        t.total = t.units * (unsigned)outer;
+        t.rows = (int)rows;
+        t.unit = unit;
+        t.first = (int)blocks;
+        blocks += (t.total + ROWS_SPAN - 1) / ROWS_SPAN;
+    }
+    return blocks > 0x7fffffffll ? PICO_ERR_SIZE : blocks;
+}
+
+PICO_API int pico_copy_rows(const long long* of, int n, const int* src, const int* dst, int pairs, cudaStream_t stream) {
+    if (n > ROWS_TENSORS || pairs < 0) return PICO_ERR_SIZE;
+    RowTensors ts;
+    const long long blocks = rows_describe(of, n, ts);
+    if (blocks < 0) return (int)blocks;
+    if (blocks == 0) return 0;
+    for (int p0 = 0; p0 < pairs; p0 += 65535) {
+        const int m = pairs - p0 < 65535 ? pairs - p0 : 65535;
+        pico_launch(copy_rows_kernel, dim3((unsigned)blocks, m), dim3(ROWS_THREADS), 0, stream, ts, src + p0, dst + p0);
+    }
+    return pico_launch_status();
+}
+
+PICO_API int pico_reorder_rows(const long long* of, int n, const int* slots, const int* parents, int groups, int places, cudaStream_t stream) {
+    if (n > ROWS_TENSORS || groups < 0 || places < 1 || places > ROWS_BEAMS) return PICO_ERR_SIZE;
+    RowTensors ts;
+    const long long blocks = rows_describe(of, n, ts);
+    if (blocks < 0) return (int)blocks;
+    if (blocks == 0) return 0;
+    for (int g0 = 0; g0 < groups; g0 += 65535) {
+        const int m = groups - g0 < 65535 ? groups - g0 : 65535;
+        pico_launch(reorder_rows_kernel, dim3((unsigned)blocks, m), dim3(ROWS_THREADS), 0, stream, ts, slots + (long long)g0 * places,
+                    parents + (long long)g0 * places, places);
+    }
+    return pico_launch_status();
+}

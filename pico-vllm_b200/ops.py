@@ -86,6 +86,10 @@ def library():
         "pico_gemm_f32_parts": [i32, i32, i32],
         "pico_tf_status": [vp],
         "pico_sample": [vp, i32, i32, i32, vp, vp, vp, vp, vp],
+        "pico_beam_select": [vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp],
+        "pico_copy_rows": [vp, i32, vp, vp, i32, vp],
+        "pico_reorder_rows": [vp, i32, vp, vp, i32, i32, vp],
+        "pico_rows_status": [vp],
         "pico_post_add_norm": [vp, vp, vp, i32, f32, vp, i32, f32, vp, vp, i32, i32, i32, i32, i32, vp],
         "pico_scale_softcap": [vp, i32, i32, i32, f32, f32, vp],
         "pico_latent_norm_store": [vp, i32, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, vp, f32, i32, i32, i32, i32, i32, vp, f32,
@@ -138,6 +142,8 @@ def library():
         fn.restype = ctypes.c_int
     lib.pico_gated_delta_chunk_floats.argtypes = [i32, i32, i32, i32]
     lib.pico_gated_delta_chunk_floats.restype = i64
+    lib.pico_beam_scratch.argtypes = [i32, i32, i32, i32, i32]
+    lib.pico_beam_scratch.restype = i64
     _lib = lib
     return lib
 
@@ -403,8 +409,9 @@ def tma_status() -> int:
 def check_kernel_status() -> None:
     """Raises KernelError when a kernel gave up a bounded wait (on a TMA copy or a tensor-core barrier)
     since the library was loaded: such a block leaves its part of the result unwritten, so the
-    tokens computed since are not to be trusted.  Reads four status words from the device (a few
-    synchronous 4-byte copies); does nothing before the library was first used."""
+    tokens computed since are not to be trusted; also when copy_pages or reorder_states met an index
+    outside a tensor.  Reads four status words from the device (a few synchronous 4-byte copies), five
+    once rows of a cache have been moved; does nothing before the library was first used."""
     if _lib is None:
         return
     bad = [name for name, word in (("paged_decode_tma (decode attention)", tma_status()),
@@ -412,6 +419,8 @@ def check_kernel_status() -> None:
                                    ("gemm_tcgen05_pair or gemm_f32_tcgen05 (products)", tc_status())) if word]
     if bad:
         raise KernelError("a bounded wait ran out in: " + ", ".join(bad) + "; results since then are invalid")
+    if _rows_used and rows_status():
+        raise KernelError("copy_pages or reorder_states met an index outside a tensor and passed it over; what was to be copied there was not")
 
 
 _PAIR_COUNTERS = {}
@@ -961,6 +970,174 @@ def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor], top_p: Opt
                                  _ptr(uniform), _ptr(out), _stream()), "sample")
     _count()
     return out
+
+
+# ------------------------------------------------------------------------------------------
+# Beam search: the choice of the beams that go on, and what of the cache has to move after it.
+BEAM_MAX = 32          # beams of a request
+_ROW_TENSORS = 16      # tensors of one launch that moves rows
+
+
+def _here(*tensors) -> None:
+    """CUDA tensors of the current device (launches go to its current stream)."""
+    _cuda(*tensors)
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t.get_device() != dev:
+            raise KernelError(f"kernel arguments must lie on the current device (cuda:{dev}), got {t.device}")
+
+
+def _span(t: torch.Tensor):
+    """First byte of a tensor and the byte behind its last."""
+    start = t.data_ptr()
+    if t.numel() == 0:
+        return start, start
+    return start, start + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a1 <= b0 or b1 <= a0
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, end_token: Optional[int] = None,
+                out: Optional[torch.Tensor] = None):
+    """One step of beam search for several requests: which beams go on, with which token, and which hypotheses end.
+
+    logits float32 [G * rows, V] (contiguous columns, any row stride): the rows of request g's beams one after the other; scores
+    float32 [G, rows]: their sums of log-probabilities.  rows is 1 .. beams (1 after a prompt), beams at most 32.  Token t of beam b is worth
+    v = scores[b] + logits[b, t] - log sum exp logits[b]; where that is a finite number (b, t) is a candidate, and candidates are ranked by v, of
+    equal ones the smaller (b, t) first.  A beam whose score is -infinity, or whose logits hold NaN or +infinity or nothing but -infinity, has none.
+
+    Returns (tokens, parents, new_scores, ended):
+    tokens, parents int32 [G, beams], new_scores float32 [G, beams]: the best ``beams`` candidates whose token is not ``end_token``, by place.  The best
+    child of beam p has place p, so that its cache can stay where it is; the others take the places that are left, in their order.
+    A place for which there is no candidate has token -1, itself as parent and the score -infinity.
+    ended float32 [G, rows]: v of (b, end_token) where that is among the best ``beams`` candidates of all, else -infinity.
+
+    All four are views of one int32 buffer (floats by their bits; in that order), which ``out`` may give: contiguous int32
+    [G * (3 * beams + rows)].  ``scores`` may be the new_scores of an earlier call with the same ``out``."""
+    if logits.dim() != 2 or scores.dim() != 2:
+        raise KernelError("beam_select: logits float32 [G * rows, V], scores float32 [G, rows]")
+    (R, V), (G, rows) = logits.shape, scores.shape
+    if logits.dtype != torch.float32 or scores.dtype != torch.float32 or R != G * rows or not scores.is_contiguous() \
+            or (V > 1 and logits.stride(1) != 1):
+        raise KernelError("beam_select: logits float32 [G * rows, V] with contiguous columns, scores contiguous float32 [G, rows]")
+    if not 1 <= beams <= BEAM_MAX or not 1 <= rows <= beams:
+        raise KernelError(f"beam_select: 1 to {BEAM_MAX} beams and no more rows than beams, got {beams} beams and {rows} rows")
+    if end_token is not None and not 0 <= end_token < V:
+        raise KernelError(f"beam_select: end token {end_token} outside [0, {V})")
+    n = G * (3 * beams + rows)
+    if out is None:
+        _here(logits, scores)
+        out = torch.empty(n, dtype=torch.int32, device=logits.device)
+    else:
+        if out.dtype != torch.int32 or out.shape != (n,) or not out.is_contiguous():
+            raise KernelError(f"beam_select: out must be contiguous int32 [{n}]")
+        _here(logits, scores, out)
+        same = rows == beams and scores.data_ptr() == out.data_ptr() + 8 * G * beams
+        if not (_apart(logits, out) and (same or _apart(scores, out))):
+            raise KernelError("beam_select: out overlaps the inputs")
+    c = G * beams
+    floats = out.view(torch.float32)
+    found = (out[:c].view(G, beams), out[c:2 * c].view(G, beams), floats[2 * c:3 * c].view(G, beams), floats[3 * c:].view(G, rows))
+    if G == 0:
+        return found
+    lib = library()
+    end = -1 if end_token is None else int(end_token)
+    need = lib.pico_beam_scratch(G, rows, V, beams, end)
+    if need < 0:
+        raise KernelError(f"beam_select: {G} requests of {rows} rows with {V} logits are more than the kernel takes")
+    scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    at = out.data_ptr()
+    _check(lib.pico_beam_select(_ptr(logits), logits.stride(0), G, rows, V, beams, end, _ptr(scores), _ptr(scratch), at, at + 4 * c,
+                                at + 8 * c, at + 12 * c, _stream()), "beam_select")
+    _count(2)
+    return found
+
+
+def _rows_of(tensors, what: str):
+    """Addresses, sizes and strides of [entries, rows, ...] tensors, 16 a launch, as the kernels that move rows take them."""
+    given = []
+    spans = []
+    for t in tensors:
+        if t.dim() < 2 or not (t.numel() == 0 or t[0, 0].is_contiguous()):
+            raise KernelError(f"{what}: tensors are [entries, rows, ...], each row of an entry in one piece")
+        E, N = t.shape[0], t.shape[1]
+        if t.numel() == 0:
+            continue
+        size = t.element_size()
+        row, outer, step = t.numel() // (E * N) * size, t.stride(0) * size, t.stride(1) * size
+        # no two rows may share a byte: rows within an entry, entries within a row's place, or one of the two alone
+        if not ((N == 1 or step >= row) and (E == 1 or outer >= step * (N - 1) + row)) \
+                and not ((E == 1 or outer >= row) and (N == 1 or step >= outer * (E - 1) + row)):
+            raise KernelError(f"{what}: rows of a tensor overlap")
+        given.append((t.data_ptr(), E, N, outer if E > 1 else 0, step if N > 1 else 0, row))
+        spans.append(_span(t))
+    spans.sort()
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise KernelError(f"{what}: tensors overlap or lie inside one another")
+    return [given[i:i + _ROW_TENSORS] for i in range(0, len(given), _ROW_TENSORS)]
+
+
+_rows_used = False
+
+
+def rows_status() -> int:
+    """0, or 1 when copy_pages or reorder_states met an index outside a tensor (and passed it over) since this was asked last."""
+    out = ctypes.c_int(0)
+    library().pico_rows_status(ctypes.addressof(out))
+    return out.value
+
+
+def copy_pages(tensors, src: torch.Tensor, dst: torch.Tensor):
+    """Copies cache pages: t[:, dst[i]] = t[:, src[i]] for every tensor t [entries, pages, ...] of the list and every i, in one launch.
+
+    Entries are layers; a page of an entry is one piece of any size and type, the strides between pages and entries may be any that keep
+    them apart.  src, dst contiguous int32 [n].  A pair with a negative index is passed over (padding of a recorded call).  No page may be
+    named twice in dst, or in dst and src both (but i with src[i] == dst[i], where nothing happens): what such pages hold afterwards is not said.
+    An index that is no page is passed over and told by ``check_kernel_status``.  Returns the list."""
+    global _rows_used
+    if src.dtype != torch.int32 or dst.dtype != torch.int32 or src.dim() != 1 or src.shape != dst.shape or not src.is_contiguous() \
+            or not dst.is_contiguous():
+        raise KernelError("copy_pages: src and dst must be contiguous int32 [n]")
+    parts = _rows_of(tensors, "copy_pages")
+    _here(src, dst, *tensors)
+    for part in parts:
+        if src.shape[0] == 0:
+            break
+        _rows_used = True
+        of = (ctypes.c_longlong * (6 * len(part)))(*[v for t in part for v in t])
+        _check(library().pico_copy_rows(ctypes.addressof(of), len(part), _ptr(src), _ptr(dst), src.shape[0], _stream()), "copy_pages")
+        _count(-(-src.shape[0] // 65535))
+    return tensors
+
+
+def reorder_states(states, slots: torch.Tensor, parents: torch.Tensor):
+    """Passes states on within groups: t[:, slots[g, p]] becomes what t[:, slots[g, parents[g, p]]] was, for every tensor t [entries, slots, ...]
+    of the list, every group g and place p, all at once and in place.
+
+    parents may be any (places that keep their own, several children of one, cycles): as ``beam_select`` gives them, or in order
+    of rank.  slots, parents contiguous int32 [G, places], at most 32 places; a place with itself as parent is left alone.  Tensors as in
+    ``copy_pages``.  No slot may be named twice, in one group or in two: what it holds afterwards is not said.  A place whose parent or
+    slot does not exist is passed over and told by ``check_kernel_status``.  Returns the list."""
+    global _rows_used
+    if slots.dtype != torch.int32 or parents.dtype != torch.int32 or slots.dim() != 2 or slots.shape != parents.shape \
+            or not slots.is_contiguous() or not parents.is_contiguous():
+        raise KernelError("reorder_states: slots and parents must be contiguous int32 [groups, places]")
+    G, places = slots.shape
+    if not 1 <= places <= BEAM_MAX:
+        raise KernelError(f"reorder_states: 1 to {BEAM_MAX} places in a group, got {places}")
+    parts = _rows_of(states, "reorder_states")
+    _here(slots, parents, *states)
+    for part in parts:
+        if G == 0:
+            break
+        _rows_used = True
+        of = (ctypes.c_longlong * (6 * len(part)))(*[v for t in part for v in t])
+        _check(library().pico_reorder_rows(ctypes.addressof(of), len(part), _ptr(slots), _ptr(parents), G, places, _stream()), "reorder_states")
+        _count(-(-G // 65535))
+    return states
 
 
 # ------------------------------------------------------------------------------------------
