@@ -12,12 +12,12 @@ __version__ = "0.1.0"
 from .errors import (PicoError, ConfigError, WeightError, OutOfPages, KernelError, ScheduleError)
 
 __all__ = ["PicoError", "ConfigError", "WeightError", "OutOfPages", "KernelError", "ScheduleError",
-           "LLM", "SamplingParams", "EngineConfig"]
+           "LLM", "SamplingParams", "BeamParams", "EngineConfig"]
 
 
 def __getattr__(name):
     # the entry points import torch and the CUDA extension; load them on first use
-    if name in ("LLM", "SamplingParams"):
+    if name in ("LLM", "SamplingParams", "BeamParams"):
         from .engine import llm
         return getattr(llm, name)
     if name == "EngineConfig":

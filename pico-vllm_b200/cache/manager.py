@@ -16,6 +16,10 @@ the last W (``commit``): the next query, at position L, reads keys L-W+1 .. L on
 The reference frees only at the end of a request (pico_vllm/cache.py:158-167) and raises when
 the pool is empty (pico_vllm/blockmanager.py:77-78); here the scheduler asks ``can_append``
 first.
+
+Requests can branch: ``fork`` gives slots that hold the same tokens, ``reorder`` passes what slots hold on
+to others (beam search), ``compact`` brings the pages in use together.  Full pages are shared and counted (the reference counts holders
+for its prefix cache only: pico_vllm/blockmanager.py:120-133; it has no beam search).
 """
 from __future__ import annotations
 
@@ -62,6 +66,7 @@ class CacheManager:
         self.groups: List[KVGroup] = []
         self.entry_group: Dict[int, tuple] = {}     # entry id -> (group index, index inside the group)
         self.states: Dict[int, torch.Tensor] = {}   # entry id -> [max_num_seqs, *shape]
+        self.state_stacks: List[torch.Tensor] = []  # [entries, max_num_seqs, *shape] each: the states of equal entries
         self.state_specs: Dict[int, object] = {}
         for eid, spec in enumerate(cache_entries):
             kind = kind_of(spec)
@@ -83,9 +88,17 @@ class CacheManager:
                 for name, page_shape in g.spec.page_tensors(page_size).items():
                     g.tensors[name] = torch.zeros((len(g.entries), num_pages) + tuple(page_shape), dtype=dtype,
                                                   device=self.device)
+            alike: Dict[tuple, List[int]] = {}
             for eid, spec in self.state_specs.items():
-                self.states[eid] = torch.zeros((max_num_seqs,) + tuple(spec.shape),
-                                               dtype=getattr(torch, spec.dtype), device=self.device)
+                alike.setdefault((tuple(spec.shape), spec.dtype), []).append(eid)
+            for (shape, dtype), eids in alike.items():
+                # states of one shape lie in one tensor, each entry on 512 bytes as if it were one of its own
+                n = max_num_seqs * int(np.prod(shape))
+                flat = torch.zeros((len(eids), -(-n // 512) * 512), dtype=getattr(torch, dtype), device=self.device)
+                stack = flat[:, :n].view((len(eids), max_num_seqs) + shape)
+                self.state_stacks.append(stack)
+                for i, eid in enumerate(eids):
+                    self.states[eid] = stack[i]
         self._free_slots = list(range(max_num_seqs - 1, -1, -1))
         self.seq_len = np.zeros(max_num_seqs, np.int64)   # tokens committed per slot
         self.pending = np.zeros(max_num_seqs, np.int64)   # tokens appended, not yet committed
@@ -104,6 +117,12 @@ class CacheManager:
     # ------------------------------------------------------------------ requests
     def acquire(self, owner=None) -> int:
         """A slot for a new request: empty block tables, zeroed state."""
+        slot = self._take_slot(owner)
+        for st in self.states.values():
+            st[slot].zero_()
+        return slot
+
+    def _take_slot(self, owner) -> int:
         if not self._free_slots:
             raise ScheduleError("no request slot is free")
         slot = self._free_slots.pop()
@@ -113,8 +132,6 @@ class CacheManager:
         for g in self.groups:
             g.first_block[slot] = 0
             g.end_block[slot] = 0
-        for st in self.states.values():
-            st[slot].zero_()
         return slot
 
     def release(self, slot: int) -> None:
@@ -133,11 +150,141 @@ class CacheManager:
         self._free_slots.append(slot)
 
     def _give_back(self, g: KVGroup, pages: List[int]) -> None:
-        freed = g.pool.release(pages)
+        self._poison(g, g.pool.release(pages))
+
+    def _poison(self, g: KVGroup, freed: List[int]) -> None:
         if self.poison_freed and freed and g.tensors:
             idx = torch.tensor(freed, dtype=torch.long, device=self.device)
             for t in g.tensors.values():
                 t[:, idx] = float("nan")
+
+    # ------------------------------------------------------------------ requests that branch
+    # Requests that hold the same tokens share the pages that are full.  The last, partly filled page is each one's own: the next token
+    # is written there.  So a page that more than one holds is never written, and what a branch costs is a copy of one page per group.
+    def fork(self, slot: int, n: int, owners: Optional[Sequence[object]] = None) -> List[int]:
+        """``n`` more slots that hold what ``slot`` does: its tokens' keys and values and its states.  All or nothing."""
+        if self.owner[slot] is None:
+            raise PicoError(f"slot {slot} is not held")
+        if self.pending[slot]:
+            raise PicoError(f"slot {slot} cannot branch: tokens appended to it are not committed")
+        if n < 0 or (owners is not None and len(owners) != n):
+            raise PicoError("one owner for each slot, and no fewer than no slots")
+        if n > len(self._free_slots):
+            raise ScheduleError(f"{n} slots wanted, {len(self._free_slots)} free")
+        L = int(self.seq_len[slot])
+        full, own = L // self.page_size, 1 if L % self.page_size else 0
+        for g in self.groups:
+            if n * own > g.pool.available:
+                raise OutOfPages(f"{n * own} pages wanted for {n} branches, {g.pool.available} of {g.pool.num_pages} free")
+        slots = [self._take_slot(None if owners is None else owners[i]) for i in range(n)]
+        if not slots:
+            return slots
+        for g in self.groups:
+            first = int(g.first_block[slot])
+            shared = g.tables[slot, first:full]
+            for s in slots:
+                g.pool.share(shared.tolist())
+                g.tables[s, first:full] = shared
+                g.first_block[s], g.end_block[s] = first, full + own
+            if own:
+                pages = g.pool.allocate(n)
+                g.tables[slots, full] = pages
+                self._copy_rows(g.tensors.values(), [int(g.tables[slot, full])] * n, pages)
+        self.seq_len[slots] = L
+        self._copy_rows(self.state_stacks, [slot] * n, slots)
+        return slots
+
+    def reorder(self, slots: Sequence[Sequence[int]], parents: Sequence[Sequence[int]], on_device=None) -> None:
+        """Passes on what requests of a family hold: slots[f][p] holds afterwards what slots[f][parents[f][p]] held, all at once, for every
+        family f.  The members of a family hold equally many tokens.  ``on_device``: (slots, parents) as int32 tensors, if
+        the caller has them there (the states are moved by them).  Needs no free page."""
+        flat = [s for line in slots for s in line]
+        if len(set(flat)) != len(flat) or len(slots) != len(parents):
+            raise PicoError("a slot belongs to one family, and every family has its parents")
+        for line, family in zip(slots, parents):
+            if len(line) != len(family) or not all(0 <= q < len(line) for q in family):
+                raise PicoError("every member of a family has a parent in it")
+            if any(self.owner[s] is None or self.pending[s] for s in line):
+                raise PicoError("a family's slots are held, and what was appended to them is committed")
+            if len({int(self.seq_len[s]) for s in line}) > 1:
+                raise PicoError("members of a family hold equally many tokens")
+        moved = [(line, family) for line, family in zip(slots, parents) if any(q != p for p, q in enumerate(family))]
+        if not moved:
+            return
+        for g in self.groups:
+            src: List[int] = []
+            dst: List[int] = []
+            gone: List[int] = []
+            for line, family in moved:
+                self._reorder_pages(g, line, family, src, dst, gone)
+            self._give_back(g, gone)
+            self._copy_rows(g.tensors.values(), src, dst)
+        if self.state_stacks:
+            from .. import ops
+            if on_device is None:
+                most = max(len(line) for line, _ in moved)
+
+                def even(lines):            # families of one size: places that are not there are their own parents
+                    return torch.tensor([list(v) + list(range(len(v), most)) for v in lines], dtype=torch.int32).to(self.device, non_blocking=True)
+                on_device = even(line for line, _ in moved), even(family for _, family in moved)
+            ops.reorder_states(self.state_stacks, *on_device)
+
+    def _reorder_pages(self, g: KVGroup, line: Sequence[int], family: Sequence[int], src: List[int], dst: List[int], gone: List[int]) -> None:
+        """One family's block tables.  Adds the pages to be copied to src and dst and those given up to gone."""
+        L = int(self.seq_len[line[0]])
+        full, first = L // self.page_size, int(g.first_block[line[0]])
+        before = g.tables[list(line), first:full + 1].copy()          # (a copy: the rows change below)
+        for p, q in enumerate(family):
+            if p != q:
+                new, old = before[q, :full - first], before[p, :full - first]
+                other = new != old
+                g.pool.share(new[other].tolist())
+                gone.extend(old[other].tolist())
+                g.tables[line[p], first:full] = new
+        if L % self.page_size == 0:
+            return
+        # the last page goes to one child (to the parent itself, where it is its own child), the others copy it to the pages of those
+        # that have none: as many as there are
+        children = set(family)
+        spare = [p for p in range(len(line)) if p not in children]
+        heirs = {q: q for q in children if family[q] == q}
+        for p, q in enumerate(family):
+            if heirs.setdefault(q, p) == p:
+                g.tables[line[p], full] = before[q, -1]
+            else:
+                page = before[spare.pop(), -1]
+                g.tables[line[p], full] = page
+                src.append(int(before[q, -1]))
+                dst.append(int(page))
+
+    def compact(self) -> int:
+        """Brings the pages in use together at the low end of every pool; returns how many were copied.  Reading keys and values of a light
+        load strewn over a large pool is slower (see PagePool)."""
+        if self.pending.any():
+            raise PicoError("pages are brought together between steps: appended tokens are not committed")
+        moved = 0
+        for g in self.groups:
+            src, dst = g.pool.gather_plan()
+            if not src:
+                continue
+            g.pool.move(src, dst)
+            to = np.arange(g.pool.num_pages, dtype=np.int32)
+            to[src] = dst
+            held = g.tables >= 0
+            g.tables[held] = to[g.tables[held]]
+            self._copy_rows(g.tensors.values(), src, dst)
+            self._poison(g, src)
+            moved += len(src)
+        return moved
+
+    def _copy_rows(self, tensors, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Rows dst of [entries, rows, ...] tensors become rows src."""
+        tensors = list(tensors)
+        if not tensors or not len(src):
+            return
+        from .. import ops
+        pairs = torch.tensor([list(src), list(dst)], dtype=torch.int32).to(self.device, non_blocking=True)
+        ops.copy_pages(tensors, pairs[0], pairs[1])
 
     # ------------------------------------------------------------------ pages for new tokens
     def _blocks_missing(self, g: KVGroup, slot: int, new_len: int) -> int:

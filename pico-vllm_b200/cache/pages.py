@@ -16,7 +16,7 @@ per page taken or given back (a fraction of a microsecond).
 from __future__ import annotations
 
 import heapq
-from typing import Iterable, List
+from typing import Iterable, List, Sequence, Tuple
 
 from ..errors import OutOfPages, PicoError
 
@@ -64,6 +64,28 @@ class PagePool:
                 heapq.heappush(self._free, p)
                 freed.append(p)
         return freed
+
+    def gather_plan(self) -> Tuple[List[int], List[int]]:
+        """(from, to): pages whose move would leave the pages in use with the lowest numbers - the highest of them, in
+        order, to the free ones below."""
+        n = self.in_use
+        to = sorted(p for p in self._free if p < n)
+        return [p for p in range(n, self.num_pages) if self._refs[p] > 0], to
+
+    def move(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Page dst[i], free so far, is held in place of src[i], by as many."""
+        if len(src) != len(dst) or len(set(src)) != len(src) or len(set(dst)) != len(dst):
+            raise PicoError("pages are moved one to one")
+        for s, d in zip(src, dst):
+            if not 0 <= s < self.num_pages or self._refs[s] < 1:
+                raise PicoError(f"page {s} is not held, it cannot be moved")
+            if not 0 <= d < self.num_pages or self._refs[d] > 0:
+                raise PicoError(f"page {d} is held, nothing can be moved there")
+        for s, d in zip(src, dst):
+            self._refs[d], self._refs[s] = self._refs[s], 0
+        taken = set(dst)
+        self._free = [p for p in self._free if p not in taken] + list(src)
+        heapq.heapify(self._free)
 
     def refcount(self, page: int) -> int:
         return self._refs[page]

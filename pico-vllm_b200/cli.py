@@ -7,7 +7,7 @@ one prompt with ``--max-new-tokens`` (20), ``--temperature`` (0 = greedy) and ``
 step until it completes and print ``[request id] output``.  Option names are the reference's
 argument names (num_gpu_blocks, block_size, max_new_tokens, temperature, top_p, use_cuda_graph,
 max_batch_size -> here the largest graph batch, max_num_seqs); options it has no name for
-(dtype, token budget, portion size, seed) are additions.
+(dtype, token budget, portion size, seed) are additions, as is ``--beams`` (beam search instead of sampling).
 
 ``python -m pico_vllm_b200.cli random-model --config CONFIG.json --seed S --out DIR`` writes a
 model folder with random weights (config.json, model.safetensors) from a configuration.
@@ -37,6 +37,13 @@ def _run(args) -> int:
     if not prompts:
         print("give at least one --prompt TEXT or --prompt-ids 1,2,3", file=sys.stderr)
         return 2
+    if args.beams is not None:
+        from . import BeamParams
+        params = BeamParams(beams=args.beams, max_new_tokens=args.max_new_tokens, length_penalty=args.length_penalty, ignore_eos=args.ignore_eos)
+        for i, out in enumerate(llm.beam_search(prompts, params)):
+            for h in out.hypotheses:
+                print(f"[{i}] {h.score:.6f} {h.text if h.text is not None else ' '.join(str(t) for t in h.token_ids)}", flush=True)
+        return 0
     for p in prompts:
         llm.submit(p, max_new_tokens=args.max_new_tokens, temperature=args.temperature, top_p=args.top_p,
                    seed=args.seed, ignore_eos=args.ignore_eos)
@@ -73,6 +80,9 @@ def main(argv=None) -> int:
     run.add_argument("--top-p", type=float, default=1.0)
     run.add_argument("--seed", type=int, default=0)
     run.add_argument("--ignore-eos", action="store_true")
+    run.add_argument("--beams", type=int, default=None, help="beam search with so many beams (needs --max-num-seqs as large); prints "
+                     "every hypothesis with its sum of log-probabilities, best first")
+    run.add_argument("--length-penalty", type=float, default=1.0)
     run.add_argument("--num-gpu-blocks", type=int, default=500)
     run.add_argument("--block-size", type=int, default=16)
     run.add_argument("--max-num-seqs", type=int, default=4)

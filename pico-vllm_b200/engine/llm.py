@@ -21,7 +21,8 @@ import torch
 from .. import ops
 from ..config.engine import EngineConfig
 from ..errors import ConfigError, ScheduleError
-from ..sampling import Sampler, SamplingParams, uniform_for
+from ..sampling import BeamParams, Sampler, SamplingParams, uniform_for
+from .beam import BeamOutput, beam_search
 from .core import make_cache, load_model
 from .runner import ModelRunner, StepItem
 from .scheduler import Request, Scheduler
@@ -126,6 +127,19 @@ class LLM:
                                       self._decode(r.generated_ids) if self.tokenizer is not None else None,
                                       r.finish_reason, r.preemptions))
         return outs
+
+    # ------------------------------------------------------------------ beam search, and the cache's pages
+    def beam_search(self, prompts: Sequence[Prompt], params: Optional[BeamParams] = None) -> List[BeamOutput]:
+        """The most likely continuations of every prompt that ``params.beams`` beams find, best first.  Prompts run side by side as far as
+        slots (one per beam) and pages allow.  No submitted request may be unfinished."""
+        if isinstance(prompts, str) or (prompts and isinstance(prompts[0], int)):
+            prompts = [prompts]
+        return beam_search(self, prompts, params if params is not None else BeamParams())
+
+    def compact_cache(self) -> int:
+        """Brings the cache's pages in use together (after a heavy load, when long requests go on); returns how many were copied.
+        Results do not change.  May be called between any two steps."""
+        return self.cache.compact()
 
     # ------------------------------------------------------------------ inside
     def _step(self) -> List[Request]:

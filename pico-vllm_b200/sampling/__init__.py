@@ -1,4 +1,4 @@
-from .params import SamplingParams
+from .params import BeamParams, SamplingParams
 from .sampler import Sampler, PendingTokens, uniform_for
 
-__all__ = ["SamplingParams", "Sampler", "PendingTokens", "uniform_for"]
+__all__ = ["SamplingParams", "BeamParams", "Sampler", "PendingTokens", "uniform_for"]

@@ -29,3 +29,27 @@ class SamplingParams:
             raise ConfigError("temperature must be >= 0 (0 means greedy)")
         if not self.top_p > 0:
             raise ConfigError("top_p must be > 0")
+
+
+@dataclass
+class BeamParams:
+    """Options of beam search: the ``beams`` best continuations are kept at every token.  A hypothesis is worth the sum of its tokens'
+    log-probabilities divided by its length to the power ``length_penalty`` (its end token counted; 0: the sum itself).  The
+    reference has no beam search."""
+    beams: int = 4
+    max_new_tokens: int = 16
+    length_penalty: float = 1.0
+    ignore_eos: bool = False
+    num_return: Optional[int] = None     # hypotheses to return, best first; None = as many as beams
+
+    def __post_init__(self):
+        if not 1 <= self.beams <= 32:
+            raise ConfigError("beams must lie in 1 .. 32")
+        if self.max_new_tokens < 1:
+            raise ConfigError("max_new_tokens must be at least 1")
+        if not 0 <= self.length_penalty < float("inf"):
+            raise ConfigError("length_penalty must be a number >= 0")
+        if self.num_return is None:
+            self.num_return = self.beams
+        if not 1 <= self.num_return <= self.beams:
+            raise ConfigError("num_return must lie in 1 .. beams")

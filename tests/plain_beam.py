@@ -54,3 +54,40 @@ def copy(t, src, dst):
         if s >= 0 and d >= 0:
             new[:, d] = t[:, s]
     return new
+
+
+def search(next_logits, prompt, beams, max_new, end_token=None, length_penalty=1.0):
+    """Beam search over ``next_logits(tokens) -> [V]``: [(value, score, tokens, reason), ..] best first, and the smallest distance of two
+    values that were compared (inputs on which rounding decides are none to test with)."""
+    found, near = [], math.inf
+    paths, scores = [[]], [0.0]
+
+    def keep(tokens, score, reason):
+        value = score / len(tokens) ** length_penalty
+        if len(found) >= beams and value <= found[-1][0]:
+            return
+        found.append((value, score, tokens, reason))
+        found.sort(key=lambda h: -h[0])
+        del found[beams:]
+    for n in range(1, max_new + 1):
+        logits = torch.stack([next_logits(prompt + p) if p is not None else torch.zeros_like(next_logits(prompt)) for p in paths])
+        tokens, parents, new, ended, ranked = select(logits.double(), torch.tensor(scores, dtype=torch.float64), beams, end_token)
+        near = min([near] + [a[0] - b[0] for a, b in zip(ranked, ranked[1:])])
+        for p, v in zip(paths, ended):
+            if v > -math.inf:
+                keep(p + [end_token], v, "eos")
+        paths = [paths[q] + [t] if t >= 0 else None for t, q in zip(tokens, parents)]
+        scores = new
+        if n == max_new:
+            for p, v in zip(paths, scores):
+                if v > -math.inf:
+                    keep(p, v, "length")
+            break
+        if max(scores) == -math.inf:
+            break
+        if len(found) >= beams:
+            gap = max(scores) / n ** length_penalty - found[-1][0]
+            near = min(near, abs(gap))
+            if gap <= 0:
+                break
+    return found, near
