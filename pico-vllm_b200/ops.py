@@ -86,7 +86,7 @@ def library():
         "pico_gemm_f32_parts": [i32, i32, i32],
         "pico_tf_status": [vp],
         "pico_sample": [vp, i32, i32, i32, vp, vp, vp, vp, vp],
-        "pico_beam_select": [vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp],
+        "pico_beam_select": [vp, i64, i32, i32, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp],
         "pico_copy_rows": [vp, i32, vp, vp, i32, vp],
         "pico_reorder_rows": [vp, i32, vp, vp, i32, i32, vp],
         "pico_rows_status": [vp],
@@ -142,8 +142,6 @@ def library():
         fn.restype = ctypes.c_int
     lib.pico_gated_delta_chunk_floats.argtypes = [i32, i32, i32, i32]
     lib.pico_gated_delta_chunk_floats.restype = i64
-    lib.pico_beam_scratch.argtypes = [i32, i32, i32, i32, i32]
-    lib.pico_beam_scratch.restype = i64
     _lib = lib
     return lib
 
@@ -980,11 +978,14 @@ _ROW_TENSORS = 16      # tensors of one launch that moves rows
 
 def _here(*tensors) -> None:
     """CUDA tensors of the current device (launches go to its current stream)."""
-    _cuda(*tensors)
-    dev = torch.cuda.current_device()
+    dev = torch.cuda.current_device() if torch.cuda.is_initialized() else None
     for t in tensors:
         if t.get_device() != dev:
-            raise KernelError(f"kernel arguments must lie on the current device (cuda:{dev}), got {t.device}")
+            _cuda(t)
+            if dev is None:
+                dev = torch.cuda.current_device()
+            if t.get_device() != dev:
+                raise KernelError(f"kernel arguments must lie on the current device (cuda:{dev}), got {t.device}")
 
 
 def _span(t: torch.Tensor):
@@ -1027,7 +1028,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, end_toke
         raise KernelError(f"beam_select: 1 to {BEAM_MAX} beams and no more rows than beams, got {beams} beams and {rows} rows")
     if end_token is not None and not 0 <= end_token < V:
         raise KernelError(f"beam_select: end token {end_token} outside [0, {V})")
-    n = G * (3 * beams + rows)
+    c, n = G * beams, G * (3 * beams + rows)
     if out is None:
         _here(logits, scores)
         out = torch.empty(n, dtype=torch.int32, device=logits.device)
@@ -1035,49 +1036,59 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, end_toke
         if out.dtype != torch.int32 or out.shape != (n,) or not out.is_contiguous():
             raise KernelError(f"beam_select: out must be contiguous int32 [{n}]")
         _here(logits, scores, out)
-        same = rows == beams and scores.data_ptr() == out.data_ptr() + 8 * G * beams
+        same = rows == beams and scores.data_ptr() == out.data_ptr() + 8 * c
         if not (_apart(logits, out) and (same or _apart(scores, out))):
             raise KernelError("beam_select: out overlaps the inputs")
-    c = G * beams
-    floats = out.view(torch.float32)
-    found = (out[:c].view(G, beams), out[c:2 * c].view(G, beams), floats[2 * c:3 * c].view(G, beams), floats[3 * c:].view(G, rows))
+    floats, at = out.view(torch.float32), out.storage_offset()
+    found = (out.as_strided((G, beams), (beams, 1), at), out.as_strided((G, beams), (beams, 1), at + c),
+             floats.as_strided((G, beams), (beams, 1), at + 2 * c), floats.as_strided((G, rows), (rows, 1), at + 3 * c))
     if G == 0:
         return found
-    lib = library()
-    end = -1 if end_token is None else int(end_token)
-    need = lib.pico_beam_scratch(G, rows, V, beams, end)
-    if need < 0:
+    if R > 65535 or rows * V > 0x7fffffff:
         raise KernelError(f"beam_select: {G} requests of {rows} rows with {V} logits are more than the kernel takes")
-    scratch = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    lists = max(R, 640)
+    scratch = torch.empty(lists * (beams if end_token is None else 2 * beams) + lists, dtype=torch.int64, device=logits.device)
     at = out.data_ptr()
-    _check(lib.pico_beam_select(_ptr(logits), logits.stride(0), G, rows, V, beams, end, _ptr(scores), _ptr(scratch), at, at + 4 * c,
-                                at + 8 * c, at + 12 * c, _stream()), "beam_select")
+    _check(library().pico_beam_select(logits.data_ptr(), logits.stride(0), G, rows, V, beams, -1 if end_token is None else int(end_token),
+                                      scores.data_ptr(), scratch.data_ptr(), lists, at, at + 4 * c, at + 8 * c, at + 12 * c, _stream()),
+           "beam_select")
     _count(2)
     return found
 
 
+_ROW_NUMBERS = [ctypes.c_longlong * (6 * n) for n in range(_ROW_TENSORS + 1)]
+
+
 def _rows_of(tensors, what: str):
-    """Addresses, sizes and strides of [entries, rows, ...] tensors, 16 a launch, as the kernels that move rows take them."""
-    given = []
-    spans = []
+    """Addresses, sizes and strides of [entries, rows, ...] tensors as the kernels that move rows take them: [(numbers, tensors), ..] a launch."""
+    numbers, spans = [], []
     for t in tensors:
-        if t.dim() < 2 or not (t.numel() == 0 or t[0, 0].is_contiguous()):
+        shape, stride = t.shape, t.stride()
+        if len(shape) < 2:
             raise KernelError(f"{what}: tensors are [entries, rows, ...], each row of an entry in one piece")
-        E, N = t.shape[0], t.shape[1]
-        if t.numel() == 0:
+        E, N = shape[0], shape[1]
+        row = 1
+        for n, s in zip(shape[:1:-1], stride[:1:-1]):
+            if s != row and n > 1 and t.numel():
+                raise KernelError(f"{what}: tensors are [entries, rows, ...], each row of an entry in one piece")
+            row *= n
+        if row == 0 or E == 0 or N == 0:
             continue
-        size = t.element_size()
-        row, outer, step = t.numel() // (E * N) * size, t.stride(0) * size, t.stride(1) * size
+        outer, step = stride[0] if E > 1 else 0, stride[1] if N > 1 else 0
         # no two rows may share a byte: rows within an entry, entries within a row's place, or one of the two alone
         if not ((N == 1 or step >= row) and (E == 1 or outer >= step * (N - 1) + row)) \
                 and not ((E == 1 or outer >= row) and (N == 1 or step >= outer * (E - 1) + row)):
             raise KernelError(f"{what}: rows of a tensor overlap")
-        given.append((t.data_ptr(), E, N, outer if E > 1 else 0, step if N > 1 else 0, row))
-        spans.append(_span(t))
-    spans.sort()
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-        raise KernelError(f"{what}: tensors overlap or lie inside one another")
-    return [given[i:i + _ROW_TENSORS] for i in range(0, len(given), _ROW_TENSORS)]
+        size, base = t.element_size(), t.data_ptr()
+        numbers += (base, E, N, outer * size, step * size, row * size)
+        spans.append((base, base + (outer * (E - 1) + step * (N - 1) + row) * size))
+    if len(spans) > 1:
+        spans.sort()
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise KernelError(f"{what}: tensors overlap or lie inside one another")
+    most = 6 * _ROW_TENSORS
+    return [(_ROW_NUMBERS[len(numbers[i:i + most]) // 6](*numbers[i:i + most]), len(numbers[i:i + most]) // 6)
+            for i in range(0, len(numbers), most)]
 
 
 _rows_used = False
@@ -1103,13 +1114,12 @@ def copy_pages(tensors, src: torch.Tensor, dst: torch.Tensor):
         raise KernelError("copy_pages: src and dst must be contiguous int32 [n]")
     parts = _rows_of(tensors, "copy_pages")
     _here(src, dst, *tensors)
-    for part in parts:
-        if src.shape[0] == 0:
-            break
+    n = src.shape[0]
+    if n and parts:
         _rows_used = True
-        of = (ctypes.c_longlong * (6 * len(part)))(*[v for t in part for v in t])
-        _check(library().pico_copy_rows(ctypes.addressof(of), len(part), _ptr(src), _ptr(dst), src.shape[0], _stream()), "copy_pages")
-        _count(-(-src.shape[0] // 65535))
+        for of, count in parts:
+            _check(library().pico_copy_rows(ctypes.addressof(of), count, src.data_ptr(), dst.data_ptr(), n, _stream()), "copy_pages")
+            _count(-(-n // 65535))
     return tensors
 
 
@@ -1130,13 +1140,11 @@ def reorder_states(states, slots: torch.Tensor, parents: torch.Tensor):
         raise KernelError(f"reorder_states: 1 to {BEAM_MAX} places in a group, got {places}")
     parts = _rows_of(states, "reorder_states")
     _here(slots, parents, *states)
-    for part in parts:
-        if G == 0:
-            break
+    if G and parts:
         _rows_used = True
-        of = (ctypes.c_longlong * (6 * len(part)))(*[v for t in part for v in t])
-        _check(library().pico_reorder_rows(ctypes.addressof(of), len(part), _ptr(slots), _ptr(parents), G, places, _stream()), "reorder_states")
-        _count(-(-G // 65535))
+        for of, count in parts:
+            _check(library().pico_reorder_rows(ctypes.addressof(of), count, slots.data_ptr(), parents.data_ptr(), G, places, _stream()), "reorder_states")
+            _count(-(-G // 65535))
     return states
 
 
