@@ -12,7 +12,7 @@
 #define BEAM_LOADS 4                                            // 16-byte loads of a thread under way
 #define BEAM_TILE (BEAM_THREADS * 4 * BEAM_LOADS)               // elements that a block takes at a time
 #define BEAM_MAX 32                                             // beams of a request: lanes of the warp that ranks
-#define BEAM_LIST (2 * BEAM_MAX + BEAM_TILE / 4 + 64)           // candidates that wait in shared memory (see beam_rows_kernel)
+#define BEAM_LIST (4 * BEAM_THREADS + 128)                      // candidates that wait in shared memory (see beam_rows_kernel)
 
 typedef unsigned long long u64;
 
@@ -34,47 +34,133 @@ __device__ __forceinline__ float beam_exp2(float x) {
     return y;
 }
 
-// Grid (parts, rows).  Block (p, r) reads elements [p * per, (p + 1) * per) of row r once (per: a multiple of the tile) and leaves their
-// largest, the sum of exp(x - largest) and their K best, in order.
-// Each thread keeps a running maximum and sum of its own elements.  Candidates wait unsorted in shared memory: an element joins them if it is above
-// `limit`, a lower bound of the K-th best so far.  Of the first tile the bound comes from maxima of groups of threads; later tiles bring a few
-// candidates each (K / j the j-th of random ones), and only when some have gathered are the K best picked out and the bound raised.
+// two sums, products at a time
+__device__ __forceinline__ u64 beam_pair(float a, float b) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 beam_unpair(u64 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ u64 beam_add2(u64 a, u64 b) {
+    u64 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ u64 beam_mul2(u64 a, u64 b) {
+    u64 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Grid (parts, rows).  Block (p, r) reads elements [p * per, (p + 1) * per) of row r (per: a multiple of the tile) and leaves their largest, the sum of
+// exp(x - largest) and their K best, in order.
+// One pass over the elements keeps, in every thread, the running maximum and sum and the maximum of each of its four columns (the 16-byte loads at
+// one place of all tiles); no thread waits for another.  The K-th largest of `groups` >= 4 K maxima of threads then bounds the K-th best from
+// below, and only the columns that reach it, a few more than K of 1,024, are read once more (from L2) for the elements themselves.
 // VEC: rows start on 16 bytes; without it the same elements go to the same threads, so that rows of equal numbers have equal sums wherever
 // they lie.
 template <bool VEC>
-__global__ void __launch_bounds__(BEAM_THREADS, 4)
+__global__ void __launch_bounds__(BEAM_THREADS, 6)
 beam_rows_kernel(const float* __restrict__ logits, long long row_stride, int V, int K, int groups, int per, u64* __restrict__ best,
                  float2* __restrict__ sums) {
     pdl_launch_dependents();
     __shared__ u64 list[BEAM_LIST];
     __shared__ u64 sorted[2 * BEAM_MAX];
-    __shared__ u64 tops[BEAM_THREADS];
+    __shared__ __align__(16) float tops[BEAM_THREADS];
+    __shared__ unsigned short columns[BEAM_THREADS * BEAM_LOADS];
     __shared__ float2 warp_sums[BEAM_THREADS / 32];
-    __shared__ int s_n;
-    __shared__ u64 s_raise;
+    __shared__ int s_n, s_columns;
+    __shared__ float s_bound;
     const int tid = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
     const int p0 = min(V, part * per), p1 = min(V, p0 + per);
     const float* x = logits + (long long)r * row_stride;
-    if (tid == 0) s_n = 0;
+    if (tid == 0) { s_n = 0; s_columns = 0; s_bound = -INFINITY; }
+    if (tid < K) sorted[tid] = 0ull;
     pdl_wait();
     constexpr float LOG2E = 1.4426950408889634f;
-    float m = -INFINITY, s = 0.f, limit = -INFINITY;
-    float next[4 * BEAM_LOADS];
-    auto fetch = [&](int t0) {
+    float m = -INFINITY, s = 0.f, column[BEAM_LOADS];
 #pragma unroll
-        for (int u = 0; u < BEAM_LOADS; ++u) {
-            const int i = t0 + (u * BEAM_THREADS + tid) * 4;
-            if (VEC && i + 3 < p1) {
-                const float4 q = __ldg(reinterpret_cast<const float4*>(x + i));
-                next[4 * u] = q.x; next[4 * u + 1] = q.y; next[4 * u + 2] = q.z; next[4 * u + 3] = q.w;
-            } else {
+    for (int u = 0; u < BEAM_LOADS; ++u) column[u] = -INFINITY;
+    auto fetch = [&](float* v, int t0) {
+        if (t0 >= p1) return;
+        if (VEC && t0 + BEAM_TILE <= p1) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) next[4 * u + e] = i + e < p1 ? __ldg(x + i + e) : -INFINITY;
+            for (int u = 0; u < BEAM_LOADS; ++u) {
+                const float4 q = __ldg(reinterpret_cast<const float4*>(x + t0 + (u * BEAM_THREADS + tid) * 4));
+                v[4 * u] = q.x; v[4 * u + 1] = q.y; v[4 * u + 2] = q.z; v[4 * u + 3] = q.w;
             }
+        } else {
+#pragma unroll
+            for (int u = 0; u < BEAM_LOADS; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = t0 + (u * BEAM_THREADS + tid) * 4 + e;
+                    v[4 * u + e] = i < p1 ? __ldg(x + i) : -INFINITY;
+                }
         }
     };
-    // the K best of the n candidates into `sorted`, in order (what is above the n-th is left as it was)
-    auto rank = [&](int n) {
+    auto take = [&](const float* v) {
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < BEAM_LOADS; ++u) {
+            const float q = fmaxf(fmaxf(v[4 * u], v[4 * u + 1]), fmaxf(v[4 * u + 2], v[4 * u + 3]));
+            column[u] = fmaxf(column[u], q);
+            tmax = fmaxf(tmax, q);
+        }
+        if (tmax > m) {
+            s *= beam_exp2((m - tmax) * LOG2E);
+            m = tmax;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        const u64 less = beam_pair(-ref, -ref), log2e = beam_pair(LOG2E, LOG2E);
+        u64 add = 0ull;
+#pragma unroll
+        for (int i = 0; i < 4 * BEAM_LOADS; i += 2) {
+            const float2 e = beam_unpair(beam_mul2(beam_add2(beam_pair(v[i], v[i + 1]), less), log2e));
+            add = beam_add2(add, beam_pair(beam_exp2(e.x), beam_exp2(e.y)));
+        }
+        const float2 halves = beam_unpair(add);
+        s += halves.x + halves.y;
+    };
+    for (int t0 = p0; t0 < p1; t0 += BEAM_TILE) {
+        float v[4 * BEAM_LOADS];
+        fetch(v, t0);
+        take(v);
+    }
+    // ---- a bound of the K-th best, and the columns that reach it
+    const int each = BEAM_THREADS / groups;
+    float top = m;
+    for (int o = 1; o < each; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (tid % each == 0) tops[tid / each] = top;
+    top = warp_max(top);
+    const float sum = warp_sum(m == -INFINITY ? s : s * beam_exp2((m - top) * LOG2E));
+    if ((tid & 31) == 0) warp_sums[tid >> 5] = make_float2(top, sum);
+    __syncthreads();
+    if (tid < groups) {
+        const float mine = tops[tid];
+        int larger = 0, equal = 0;
+#pragma unroll 4
+        for (int j = 0; j < groups; j += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(tops + j);
+            larger += (q.x > mine) + (q.y > mine) + (q.z > mine) + (q.w > mine);
+            equal += (q.x == mine) + (q.y == mine) + (q.z == mine) + (q.w == mine);
+        }
+        if (larger < K && larger + equal >= K) s_bound = mine;
+    }
+    __syncthreads();
+    const float bound = s_bound;
+#pragma unroll
+    for (int u = 0; u < BEAM_LOADS; ++u)
+        if (column[u] >= bound && column[u] > -INFINITY) columns[atomicAdd(&s_columns, 1)] = (unsigned short)(u * BEAM_THREADS + tid);
+    __syncthreads();
+    // ---- their elements; after every 256 loads there is room for all that the next ones may bring
+    const int tiles = (p1 - p0 + BEAM_TILE - 1) / BEAM_TILE, loads = s_columns * tiles;
+    u64 least = 0ull;
+    auto rank = [&](int n) {                // the K best of the n candidates into `sorted`, in order
         for (int i = tid; i < n; i += BEAM_THREADS) {
             const u64 mine = list[i];
             int better = 0;
@@ -84,106 +170,43 @@ beam_rows_kernel(const float* __restrict__ logits, long long row_stride, int V, 
         }
         __syncthreads();
     };
-    int gathered = 0, room = BEAM_LIST;     // candidates since the last ranking, about; places of the list that are free, at least
-    if (p0 < p1) fetch(p0);
-    for (int t0 = p0; t0 < p1; t0 += BEAM_TILE) {
-        float v[4 * BEAM_LOADS];
+    for (int l0 = 0; l0 < loads; l0 += BEAM_THREADS) {
+        const int l = l0 + tid;
+        if (l < loads) {
+            const int c = l / tiles, i = p0 + (l - c * tiles) * BEAM_TILE + columns[c] * 4;
+            float v[4];
+            if (VEC && i + 4 <= p1) {
+                const float4 q = __ldg(reinterpret_cast<const float4*>(x + i));
+                v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+            } else {
 #pragma unroll
-        for (int i = 0; i < 4 * BEAM_LOADS; ++i) v[i] = next[i];
-        if (t0 + BEAM_TILE < p1) fetch(t0 + BEAM_TILE);
-        float tmax = v[0];
-#pragma unroll
-        for (int i = 1; i < 4 * BEAM_LOADS; ++i) tmax = fmaxf(tmax, v[i]);
-        if (tmax > m) {
-            s *= beam_exp2((m - tmax) * LOG2E);
-            m = tmax;
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float add = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4 * BEAM_LOADS; ++i) add += beam_exp2((v[i] - ref) * LOG2E);
-        s += add;
-        // ---- candidates (later elements lose to equal earlier ones: what is not above the bound is none)
-        const int above = __syncthreads_count(tmax > limit);
-        if (above == 0) continue;
-        u64 raise = 0ull;
-        int most = 4 * BEAM_LOADS * above;
-        if (above > K) {
-            // many: the K-th largest of `groups` >= 4 K maxima, each of as many threads, bounds the K-th best from below, and at most
-            // (K - 1) * TILE / groups + 1 <= TILE / 4 elements reach it
-            u64 top = 0ull;
-            if (tmax > limit) {
-#pragma unroll
-                for (int i = 4 * BEAM_LOADS - 1; i >= 0; --i)
-                    if (v[i] == tmax) top = beam_key(tmax, t0 + ((i >> 2) * BEAM_THREADS + tid) * 4 + (i & 3));
+                for (int e = 0; e < 4; ++e) v[e] = i + e < p1 ? __ldg(x + i + e) : -INFINITY;
             }
-            const int each = BEAM_THREADS / groups;
-            for (int o = 1; o < each; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (tid % each == 0) tops[tid / each] = top;
-            if (tid == 0) s_raise = 0ull;
-            __syncthreads();
-            if (tid < groups) {
-                const u64 mine = tops[tid];
-                int better = 0;
-#pragma unroll 8
-                for (int j = 0; j < groups; ++j) better += tops[j] > mine;
-                if (better == K - 1 && mine) s_raise = mine;
-            }
-            __syncthreads();
-            raise = s_raise;
-            most = BEAM_TILE / 4;
-        }
-        if (most > room) {                  // pick out the K best first
-            const int n = s_n;
-            rank(n);
-            if (tid < min(n, K)) list[tid] = sorted[tid];
-            if (tid == 0) s_n = min(n, K);
-            if (n >= K) limit = fmaxf(limit, beam_key_logit(sorted[K - 1]));
-            gathered = 0;
-            room = BEAM_LIST - K;
-            __syncthreads();
-        }
-        if (tmax > limit) {
 #pragma unroll
-            for (int i = 0; i < 4 * BEAM_LOADS; ++i)
-                if (v[i] > limit) {
-                    const u64 key = beam_key(v[i], t0 + ((i >> 2) * BEAM_THREADS + tid) * 4 + (i & 3));
-                    if (key >= raise) list[atomicAdd(&s_n, 1)] = key;
+            for (int e = 0; e < 4; ++e)
+                if (v[e] >= bound && v[e] > -INFINITY) {
+                    const u64 key = beam_key(v[e], i + e);
+                    if (key > least) list[atomicAdd(&s_n, 1)] = key;
                 }
         }
-        room -= most;
-        gathered += min(above, 2 * K);
-        if (raise) limit = beam_key_logit(raise);
-        if (gathered > 3 * K) {
+        __syncthreads();
+        const int n = s_n;
+        if (l0 + BEAM_THREADS < loads && n > BEAM_LIST - 4 * BEAM_THREADS) {
+            rank(n);
+            if (tid < K) list[tid] = sorted[tid];
+            if (tid == 0) s_n = K;
+            least = sorted[K - 1];
             __syncthreads();
-            const int n = s_n;
-            if (n > K) {
-                rank(n);
-                limit = fmaxf(limit, beam_key_logit(sorted[K - 1]));
-                if (tid < K) list[tid] = sorted[tid];
-                if (tid == 0) s_n = K;
-            }
-            gathered = 0;
-            room = BEAM_LIST - min(n, K);
-            // (the barrier before the next candidates is the next tile's)
         }
     }
-    // ---- the part's results
-    float top = warp_max(m);
-    float sum = warp_sum(m == -INFINITY ? s : s * beam_exp2((m - top) * LOG2E));
-    if ((tid & 31) == 0) warp_sums[tid >> 5] = make_float2(top, sum);
-    __syncthreads();
-    const int n = s_n;
-    if (tid < K) sorted[tid] = 0ull;
-    __syncthreads();
-    rank(n);
+    rank(s_n);
     const size_t at = (size_t)r * gridDim.x + part;
     if (tid < K) best[at * K + tid] = sorted[tid];
     if (tid < 32) {
         const float2 q = tid < BEAM_THREADS / 32 ? warp_sums[tid] : make_float2(-INFINITY, 0.f);
-        top = warp_max(q.x);
-        sum = warp_sum(q.x == -INFINITY ? q.y : q.y * beam_exp2((q.x - top) * LOG2E));
-        if (tid == 0) sums[at] = make_float2(top, sum);
+        const float all = warp_max(q.x);
+        const float total = warp_sum(q.x == -INFINITY ? q.y : q.y * beam_exp2((q.x - all) * LOG2E));
+        if (tid == 0) sums[at] = make_float2(all, total);
     }
 }
 
@@ -201,109 +224,60 @@ __device__ __forceinline__ u64 beam_order(double v) {
 }
 __device__ __forceinline__ double beam_unorder(u64 o) { return __longlong_as_double((long long)(o >> 63 ? o & 0x7fffffffffffffffull : ~o)); }
 
-// Grid (groups), a warp for each of the group's rows (four at least: all of them fetch).  Warp b merges the lists of row b's parts, a lane for every
-// 32nd of them, then the first warp ranks the rows' lists against one another, a lane for each row, until B candidates that go on are found: what a
-// round waits for are the two warp-wide maxima and the winner's next number, which is there already.
+// Grid (groups), a warp for each of the group's rows.  Warp b merges the lists of row b's parts, a lane for each, then the first warp ranks the rows'
+// lists against one another, a lane for each row, until B candidates that go on are found.  What a round waits for are the two warp-wide
+// maxima and the winner's next number, which is there already.  The kernel is all latency, of its instructions too: it is kept short.
 __global__ void beam_join_kernel(const u64* __restrict__ best, const float2* __restrict__ sums, int parts, int K, int rows, int beams, int end_token,
                                  const float* scores, int* tokens, int* parents, float* out_scores, float* ended) {
     pdl_launch_dependents();
     __shared__ u64 values[BEAM_MAX][2 * BEAM_MAX];              // of the rows' best, in order
     __shared__ int places[BEAM_MAX][2 * BEAM_MAX];              // their tokens
     __shared__ int ends[BEAM_MAX];                              // which of them is the end token
-    extern __shared__ __align__(16) unsigned char beam_smem[];
-    u64* keys = reinterpret_cast<u64*>(beam_smem);                                       // [rows][parts][K]
-    unsigned char* heads = beam_smem + (size_t)rows * parts * K * sizeof(u64);           // [rows][parts]: how many of a list are taken
+    extern __shared__ __align__(16) u64 beam_keys[];            // [rows][parts][K]
     const int g = blockIdx.x, lane = threadIdx.x & 31, b = threadIdx.x >> 5;
     pdl_wait();
     {
-        const u64* from = best + (size_t)g * rows * parts * K;
-        const unsigned to = (unsigned)__cvta_generic_to_shared(keys);
-#pragma unroll 8
-        for (int i = threadIdx.x; i < rows * parts * K; i += blockDim.x)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to + 8u * i), "l"(from + i) : "memory");
-    }
-    double off = 0.0, row_top = 0.0;
-    if (b < rows) {
+        const size_t row = (size_t)g * rows + b;
+        u64* mine = beam_keys + (size_t)b * parts * K;
+        const unsigned to = (unsigned)__cvta_generic_to_shared(mine);
+#pragma unroll 1
+        for (int i = lane; i < parts * K; i += 32)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to + 8u * i), "l"(best + row * parts * K + i) : "memory");
+        const float2 c = lane < parts ? sums[row * parts + lane] : make_float2(-INFINITY, 0.f);
+        const float score = scores[row];
+        const float top = warp_max(c.x);
+        const float sum = warp_sum(c.x == -INFINITY ? c.y : c.y * beam_exp2((c.x - top) * 1.4426950408889634f));
+        // log(f * 2^n), f in [1, 2): the whole part in 64 bits, so that the result is off by the rounding of a number below 0.7
+        const int n = (int)(__float_as_uint(sum) >> 23) - 127;
+        const float f = __uint_as_float((__float_as_uint(sum) & 0x007fffffu) | 0x3f800000u);
         // v = (x - largest) + (s - log sum): as near to s as it gets, however large the logits are
-        const float2* q = sums + ((size_t)g * rows + b) * parts;
-        const float score = scores[g * rows + b];
-        float top = -INFINITY;
-        double sum = 0.0;
-#pragma unroll 2
-        for (int p = lane; p < parts; p += 32) {
-            const float2 c = q[p];
-            if (c.x > top) {
-                sum *= (double)expf(top - c.x);
-                top = c.x;
-            }
-            sum += c.x == -INFINITY ? (double)c.y : (double)c.y * (double)expf(c.x - top);
-        }
-        const float all = warp_max(top);
-        if (top != -INFINITY) sum *= (double)expf(top - all);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        off = (double)score - log(sum);
-        row_top = (double)all;
-    }
-    asm volatile("cp.async.wait_all;\n" ::: "memory");
-    __syncthreads();
-    if (b < rows) {
-        u64* mine = keys + (size_t)b * parts * K;
-        u64* out = values[b];
-        if (!isfinite(off)) {
-            for (int k = lane; k < K; k += 32) out[k] = 0ull;
-        } else if (parts == 1) {
-            for (int k = lane; k < K; k += 32) out[k] = mine[k];
-        } else if (parts <= 64) {
-            const u64 *q0 = mine + lane * K, *q1 = q0 + 32 * K;
-            const bool has0 = lane < parts, has1 = lane + 32 < parts;
-            int k0 = 0, k1 = 0;
-            u64 c0 = has0 ? q0[0] : 0ull, c1 = has1 ? q1[0] : 0ull, d0 = has0 && K > 1 ? q0[1] : 0ull, d1 = has1 && K > 1 ? q1[1] : 0ull;
-            for (int k = 0; k < K; ++k) {
-                const u64 w = beam_warp_max(max(c0, c1));
-                if (lane == 0) out[k] = w;
-                if (w == 0ull) continue;
-                if (c0 == w) {
-                    c0 = d0;
-                    ++k0;
-                    d0 = k0 + 1 < K ? q0[k0 + 1] : 0ull;
-                } else if (c1 == w) {
-                    c1 = d1;
-                    ++k1;
-                    d1 = k1 + 1 < K ? q1[k1 + 1] : 0ull;
-                }
-            }
-        } else {
-            unsigned char* taken = heads + b * parts;
-            for (int p = lane; p < parts; p += 32) taken[p] = 0;
-            u64 head = 0ull;
-            int from = 0;
-            auto look = [&]() {
-                head = 0ull;
-                for (int p = lane; p < parts; p += 32) {
-                    const u64 c = taken[p] < K ? mine[p * K + taken[p]] : 0ull;
-                    if (c > head) { head = c; from = p; }
-                }
-            };
-            look();
-            for (int k = 0; k < K; ++k) {
-                const u64 w = beam_warp_max(head);
-                if (lane == 0) out[k] = w;
-                if (w != 0ull && head == w) {
-                    ++taken[from];
-                    look();
-                }
-            }
-        }
+        const double off = (double)score - ((double)n * 0.69314718055994530942 + (double)logf(f));
+        // (a row with an infinity or without any number: its sum is none or 0)
+        const bool dead = !(sum > 0.f && sum < INFINITY) || !isfinite(score);
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
         __syncwarp();
+        const u64* q = mine + lane * K;
+        int k = 0;
+        u64 head = lane < parts && !dead ? q[0] : 0ull, next = lane < parts && !dead && K > 1 ? q[1] : 0ull;
+#pragma unroll 1
+        for (int j = 0; j < K; ++j) {
+            const u64 w = beam_warp_max(head);
+            if (lane == 0) values[b][j] = w;
+            if (w != 0ull && head == w) {
+                head = next;
+                ++k;
+                next = k + 1 < K ? q[k + 1] : 0ull;
+            }
+        }
         if (lane == 0) ends[b] = -1;
         __syncwarp();
-        for (int k = lane; k < K; k += 32) {
-            const u64 key = out[k];
+#pragma unroll 1
+        for (int j = lane; j < K; j += 32) {
+            const u64 key = values[b][j];
             const int t = beam_key_at(key);
-            out[k] = key ? beam_order(((double)beam_key_logit(key) - row_top) + off) : 0ull;
-            places[b][k] = t;
-            if (key && t == end_token) ends[b] = k;
+            values[b][j] = key ? beam_order(((double)beam_key_logit(key) - (double)top) + off) : 0ull;
+            places[b][j] = t;
+            if (key && t == end_token) ends[b] = j;
         }
     }
     __syncthreads();
@@ -357,10 +331,12 @@ __global__ void beam_join_kernel(const u64* __restrict__ best, const float2* __r
 
 #define BEAM_JOIN_KEYS 20480    // candidates that a block of beam_join_kernel has room for in shared memory (160 KB)
 
-// Parts of a row: as many as run at once over all rows, none shorter than a tile, and no more than the join and the scratch have room for.
+// Parts of a row: as many as run at once over all rows (256 rows of 151,936 in 1 / 2 / 3 / 4 / 7 parts: 44 / 43 / 35 / 42 / 36 us with the join; four rows in
+// 7 / 10 / 19: 8.9 / 8.3 / 7.6), none shorter than a tile, and no more than the join (a lane each) and the scratch have room for.
 static int beam_parts(int groups, int rows, int V, int K, long long lists) {
     const int tiles = (V + BEAM_TILE - 1) / BEAM_TILE, R = groups * rows;
-    long long want = (4 * pico_num_sms()) / R;
+    long long want = (6 * pico_num_sms()) / R;
+    if (want > 32) want = 32;
     if (want > BEAM_JOIN_KEYS / (rows * K)) want = BEAM_JOIN_KEYS / (rows * K);
     if (want > lists / R) want = lists / R;
     const int parts = want < 1 ? 1 : want > tiles ? tiles : (int)want;
@@ -370,7 +346,7 @@ static int beam_parts(int groups, int rows, int V, int K, long long lists) {
 
 // logits: [groups * rows, row_stride] float32, the first V columns are used; scores: [groups, rows].  tokens, parents, out_scores: [groups, beams];
 // ended: [groups, rows].  end_token < 0: none.  out_scores may be scores where rows == beams.
-// scratch: `lists` lists of 16 * beams + 8 bytes (8 * beams + 8 without an end token), from a 16-byte boundary on; one for each row at least, and 640 let
+// scratch: `lists` lists of 16 * beams + 8 bytes (8 * beams + 8 without an end token), from a 16-byte boundary on; one for each row at least, and 960 let
 // rows be read in as many parts as a device of 160 multiprocessors runs at once.
 PICO_API int pico_beam_select(const float* logits, long long row_stride, int groups, int rows, int V, int beams, int end_token, const float* scores,
                               void* scratch, int lists, int* tokens, int* parents, float* out_scores, float* ended, cudaStream_t stream) {
@@ -384,16 +360,15 @@ PICO_API int pico_beam_select(const float* logits, long long row_stride, int gro
     u64* best = reinterpret_cast<u64*>(scratch);
     float2* sums = reinterpret_cast<float2*>(best + (size_t)R * parts * K);
     const bool vec = row_stride % 4 == 0 && ((uintptr_t)logits & 15) == 0;
-    const size_t smem = (size_t)rows * parts * (K * sizeof(u64) + 1);
+    const size_t smem = (size_t)rows * parts * K * sizeof(u64);
     if (smem > 20 * 1024) {             // beside the kernel's own 25 KB
         const cudaError_t e = cudaFuncSetAttribute(beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)cudaGetLastError();
     }
-    if (vec) pico_launch(beam_rows_kernel<true>, dim3(parts, R), dim3(BEAM_THREADS), 0, stream, logits, row_stride, V, K, sets, per, best, sums);
-    else pico_launch(beam_rows_kernel<false>, dim3(parts, R), dim3(BEAM_THREADS), 0, stream, logits, row_stride, V, K, sets, per, best, sums);
+    pico_launch(vec ? beam_rows_kernel<true> : beam_rows_kernel<false>, dim3(parts, R), dim3(BEAM_THREADS), 0, stream, logits, row_stride, V, K, sets, per, best, sums);
     const int status = pico_launch_status();
     if (status) return status;
-    pico_launch(beam_join_kernel, dim3(groups), dim3(32 * (rows < 4 ? 4 : rows)), smem, stream, (const u64*)best, (const float2*)sums, parts, K, rows, beams, end_token,
+    pico_launch(beam_join_kernel, dim3(groups), dim3(32 * rows), smem, stream, (const u64*)best, (const float2*)sums, parts, K, rows, beams, end_token,
                 scores, tokens, parents, out_scores, ended);
     return pico_launch_status();
 }

@@ -1046,7 +1046,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, end_toke
         return found
     if R > 65535 or rows * V > 0x7fffffff:
         raise KernelError(f"beam_select: {G} requests of {rows} rows with {V} logits are more than the kernel takes")
-    lists = max(R, 640)
+    lists = max(R, 960)
     scratch = torch.empty(lists * (beams if end_token is None else 2 * beams) + lists, dtype=torch.int64, device=logits.device)
     at = out.data_ptr()
     _check(library().pico_beam_select(logits.data_ptr(), logits.stride(0), G, rows, V, beams, -1 if end_token is None else int(end_token),
