@@ -2,13 +2,15 @@
 // come of them.  Nothing is computed: what bounds both is reading every row that is copied once and writing every row that is overwritten once.
 //
 // A tensor is [outer, rows, ...] with the bytes of a row in one piece; "row r" is the rows r of all its outer entries (a page of every layer, the
-// state of a request in every layer).  Sizes, strides and starts may be any: 16 bytes go at a time where all of them allow it, else 8, 4, 2 or 1.
+// state of a request in every layer).  Sizes, strides and starts may be any: 16 bytes go at a time where all of them allow it.
 #include "common.cuh"
 
 #define ROWS_TENSORS 16                                         // tensors of one launch
 #define ROWS_THREADS 256
 #define ROWS_LOADS 4                                            // loads of a thread under way
 #define ROWS_SPAN (ROWS_THREADS * ROWS_LOADS)                   // units of a block
+#define SHIFT_LOADS 2                                           // ... where words are put together
+#define SHIFT_SPAN (ROWS_THREADS * SHIFT_LOADS)
 #define ROWS_BEAMS 32                                           // places of a group: lanes of a warp
 
 __device__ int g_rows_status = 0;    // 0 = fine; 1 = an index outside a tensor was passed over
@@ -21,9 +23,9 @@ PICO_API int pico_rows_status(int* out) {
 
 struct RowTensor {
     char* base;
-    long long outer_stride, row_stride;  // bytes
+    long long outer_stride, row_stride, bytes;   // bytes: of a row
     unsigned units, total;               // of a row; of a row in all outer entries
-    int rows, unit;                      // unit: bytes
+    int rows, unit;                      // unit: bytes that go at a time (in copy_shifted: that every start and size is a multiple of)
     int first;                           // the first block (x) that works on this tensor
 };
 struct RowTensors {
@@ -31,37 +33,95 @@ struct RowTensors {
     int n, rows;                         // rows: the fewest that one of them has
 };
 
-// The place of unit i of row 0.
-__device__ __forceinline__ long long row_unit(const RowTensor& t, unsigned i) {
-    const unsigned o = i / t.units;
-    return (long long)o * t.outer_stride + (long long)(i - o * t.units) * t.unit;
-}
 __device__ __forceinline__ int rows_tensor(const RowTensors& ts, int block) {
     int k = 0;
     while (k + 1 < ts.n && block >= ts.t[k + 1].first) ++k;
     return k;
 }
 
-template <typename U>
-__device__ __forceinline__ void copy_units(const RowTensor& t, int block, int src, int dst) {
+__device__ __forceinline__ void copy_aligned(const RowTensor& t, int block, int src, int dst) {
     const long long from = (long long)src * t.row_stride, to = (long long)dst * t.row_stride;
     const unsigned i0 = (unsigned)block * ROWS_SPAN + threadIdx.x;
-    U v[ROWS_LOADS];
+    uint4 v[ROWS_LOADS];
     long long at[ROWS_LOADS];
 #pragma unroll
     for (int u = 0; u < ROWS_LOADS; ++u) {
         const unsigned i = i0 + u * ROWS_THREADS;
         if (i < t.total) {
-            at[u] = row_unit(t, i);
-            v[u] = *reinterpret_cast<const U*>(t.base + at[u] + from);
+            const unsigned o = i / t.units;
+            at[u] = (long long)o * t.outer_stride + (i - o * t.units) * 16ll;
+            v[u] = *reinterpret_cast<const uint4*>(t.base + at[u] + from);
         }
     }
 #pragma unroll
     for (int u = 0; u < ROWS_LOADS; ++u)
-        if (i0 + u * ROWS_THREADS < t.total) *reinterpret_cast<U*>(t.base + at[u] + to) = v[u];
+        if (i0 + u * ROWS_THREADS < t.total) *reinterpret_cast<uint4*>(t.base + at[u] + to) = v[u];
+}
+
+// The same for rows that start anywhere: the bytes of row dst are stored in whole 16-byte words, cut from the two words of row src that hold them; what
+// is the row's of its first and last word goes in bytes or pairs of them.  Only words that hold bytes of the row are read.  (t.units: the words
+// that a row may touch.)
+__device__ __forceinline__ void copy_shifted(const RowTensor& t, int block, int src, int dst) {
+    const unsigned i0 = (unsigned)block * SHIFT_SPAN + threadIdx.x;
+    uint4 lo[SHIFT_LOADS], hi[SHIFT_LOADS];
+    char* to[SHIFT_LOADS];
+    int first[SHIFT_LOADS], last[SHIFT_LOADS], shift[SHIFT_LOADS];                     // the word's bytes first .. last - 1 are the row's
+#pragma unroll
+    for (int u = 0; u < SHIFT_LOADS; ++u) {
+        const unsigned i = i0 + u * ROWS_THREADS, o = i / t.units;
+        char* row = t.base + (long long)o * t.outer_stride;
+        char* d = row + (long long)dst * t.row_stride;
+        to[u] = reinterpret_cast<char*>((uintptr_t)d & ~(uintptr_t)15) + (i - o * t.units) * 16ll;
+        const long long before = d - to[u], behind = d + t.bytes - to[u];             // where the row starts and ends, from the word
+        first[u] = before > 0 ? (int)before : 0;
+        last[u] = i < t.total && behind > first[u] ? (behind < 16 ? (int)behind : 16) : 0;
+        shift[u] = 0;
+        if (last[u] > first[u]) {
+            const char* from = row + (long long)src * t.row_stride - before;        // what belongs at to[u]
+            shift[u] = (int)((uintptr_t)from & 15);
+            const char* word = from - shift[u];
+            if (first[u] + shift[u] < 16) lo[u] = *reinterpret_cast<const uint4*>(word);
+            if (last[u] + shift[u] > 16) hi[u] = *reinterpret_cast<const uint4*>(word + 16);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < SHIFT_LOADS; ++u) {
+        if (last[u] <= first[u]) continue;
+        unsigned w[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+        if (shift[u] & 8) {
+#pragma unroll
+            for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+        }
+        if (shift[u] & 4) {
+#pragma unroll
+            for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+        }
+        uint4 v;
+        const int bits = (shift[u] & 3) * 8;
+        v.x = __funnelshift_r(w[0], w[1], bits);
+        v.y = __funnelshift_r(w[1], w[2], bits);
+        v.z = __funnelshift_r(w[2], w[3], bits);
+        v.w = __funnelshift_r(w[3], w[4], bits);
+        if (first[u] == 0 && last[u] == 16) *reinterpret_cast<uint4*>(to[u]) = v;
+        else {
+            const unsigned q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+                const unsigned b = q[k / 4] >> (k % 4 * 8);
+                if (t.unit == 1) {
+                    if (k >= first[u] && k < last[u]) to[u][k] = (char)b;
+                    if (k + 1 >= first[u] && k + 1 < last[u]) to[u][k + 1] = (char)(b >> 8);
+                } else if (k >= first[u] && k < last[u]) {
+                    *reinterpret_cast<unsigned short*>(to[u] + k) = (unsigned short)b;
+                }
+            }
+        }
+    }
 }
 
 // Grid (blocks of a row over all tensors, pairs): row dst[y] becomes row src[y].  A pair with a negative index, or of a row with itself, is passed over.
+// SHIFTED: sizes, strides and starts that are no multiples of 16 bytes.  1,201 rows of 9 x 1,358 bytes in pairs of bytes take 16.1 us, so 9.2.
+template <bool SHIFTED>
 __global__ void __launch_bounds__(ROWS_THREADS) copy_rows_kernel(RowTensors ts, const int* __restrict__ src, const int* __restrict__ dst) {
     pdl_launch_dependents();
     const RowTensor t = ts.t[rows_tensor(ts, blockIdx.x)];
@@ -72,12 +132,8 @@ __global__ void __launch_bounds__(ROWS_THREADS) copy_rows_kernel(RowTensors ts, 
         if (threadIdx.x == 0) g_rows_status = 1;
         return;
     }
-    const int block = blockIdx.x - t.first;
-    if (t.unit == 16) copy_units<uint4>(t, block, s, d);
-    else if (t.unit == 8) copy_units<uint2>(t, block, s, d);
-    else if (t.unit == 4) copy_units<unsigned>(t, block, s, d);
-    else if (t.unit == 2) copy_units<unsigned short>(t, block, s, d);
-    else copy_units<unsigned char>(t, block, s, d);
+    if (SHIFTED) copy_shifted(t, blockIdx.x - t.first, s, d);
+    else copy_aligned(t, blockIdx.x - t.first, s, d);
 }
 
 // What a group's blocks have to do, in order: row to[i] becomes row from[i].  from -1: the row that was put aside; to -1: puts the row aside.
@@ -172,9 +228,12 @@ __global__ void __launch_bounds__(ROWS_THREADS) reorder_rows_kernel(RowTensors t
     else move_units<unsigned char>(t, piece, moves, aside);
 }
 
+// How a launch divides rows: in blocks of 16-byte units over all outer entries (aligned tensors, or the others), or in pieces within an entry.
+enum RowWork { ROWS_ALIGNED, ROWS_SHIFTED, ROWS_PIECES };
+
 // What a launch needs to know of n tensors.  of: six numbers for each - address, outer entries, rows, bytes between outer entries, bytes between rows, bytes
-// of a row.  Returns the blocks (x) of the launch, or a negative code.
-static long long rows_describe(const long long* of, int n, RowTensors& ts, bool pieces) {
+// of a row.  Tensors that are not for this kind of work are left out.  Returns the blocks (x) of the launch, or a negative code.
+static long long rows_describe(const long long* of, int n, RowTensors& ts, RowWork work) {
     ts.n = 0;
     ts.rows = 0x7fffffff;
     long long blocks = 0;
@@ -184,31 +243,36 @@ static long long rows_describe(const long long* of, int n, RowTensors& ts, bool 
         if (rows > 0x7fffffffll || outer_stride < 0 || row_stride < 0) return PICO_ERR_SIZE;
         const long long all = base | bytes | (outer > 1 ? outer_stride : 0) | (rows > 1 ? row_stride : 0);
         const int unit = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
-        if (bytes / unit > 0x7fffffffll / outer) return PICO_ERR_SIZE;
+        if (work != ROWS_PIECES && (unit == 16) != (work == ROWS_ALIGNED)) continue;
+        const long long units = work == ROWS_SHIFTED ? (bytes + 30) / 16 : bytes / unit;
+        if (units > 0x7fffffffll / outer) return PICO_ERR_SIZE;
         RowTensor& t = ts.t[ts.n++];
         t.base = reinterpret_cast<char*>(base);
         t.outer_stride = outer_stride;
         t.row_stride = row_stride;
-        t.units = (unsigned)(bytes / unit);
+        t.bytes = bytes;
+        t.units = (unsigned)units;
         t.total = t.units * (unsigned)outer;
         t.rows = (int)rows;
         if (t.rows < ts.rows) ts.rows = t.rows;
         t.unit = unit;
         t.first = (int)blocks;
-        blocks += pieces ? outer * ((t.units + ROWS_SPAN - 1) / ROWS_SPAN) : (t.total + ROWS_SPAN - 1) / ROWS_SPAN;
+        const int span = work == ROWS_SHIFTED ? SHIFT_SPAN : ROWS_SPAN;
+        blocks += work == ROWS_PIECES ? outer * ((units + span - 1) / span) : (t.total + span - 1ll) / span;
+        if (blocks > 0x7fffffffll) return PICO_ERR_SIZE;
     }
-    return blocks > 0x7fffffffll ? PICO_ERR_SIZE : blocks;
+    return blocks;
 }
 
 PICO_API int pico_copy_rows(const long long* of, int n, const int* src, const int* dst, int pairs, cudaStream_t stream) {
     if (n > ROWS_TENSORS || pairs < 0) return PICO_ERR_SIZE;
-    RowTensors ts;
-    const long long blocks = rows_describe(of, n, ts, false);
-    if (blocks < 0) return (int)blocks;
-    if (blocks == 0) return 0;
+    RowTensors aligned, shifted;
+    const long long a = rows_describe(of, n, aligned, ROWS_ALIGNED), b = rows_describe(of, n, shifted, ROWS_SHIFTED);
+    if (a < 0 || b < 0) return PICO_ERR_SIZE;
     for (int p0 = 0; p0 < pairs; p0 += 65535) {
         const int m = pairs - p0 < 65535 ? pairs - p0 : 65535;
-        pico_launch(copy_rows_kernel, dim3((unsigned)blocks, m), dim3(ROWS_THREADS), 0, stream, ts, src + p0, dst + p0);
+        if (a) pico_launch(copy_rows_kernel<false>, dim3((unsigned)a, m), dim3(ROWS_THREADS), 0, stream, aligned, src + p0, dst + p0);
+        if (b) pico_launch(copy_rows_kernel<true>, dim3((unsigned)b, m), dim3(ROWS_THREADS), 0, stream, shifted, src + p0, dst + p0);
     }
     return pico_launch_status();
 }
@@ -216,7 +280,7 @@ PICO_API int pico_copy_rows(const long long* of, int n, const int* src, const in
 PICO_API int pico_reorder_rows(const long long* of, int n, const int* slots, const int* parents, int groups, int places, cudaStream_t stream) {
     if (n > ROWS_TENSORS || groups < 0 || places < 1 || places > ROWS_BEAMS) return PICO_ERR_SIZE;
     RowTensors ts;
-    const long long blocks = rows_describe(of, n, ts, true);
+    const long long blocks = rows_describe(of, n, ts, ROWS_PIECES);
     if (blocks < 0) return (int)blocks;
     if (blocks == 0) return 0;
     for (int g0 = 0; g0 < groups; g0 += 65535) {

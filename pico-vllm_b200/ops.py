@@ -1060,8 +1060,9 @@ _ROW_NUMBERS = [ctypes.c_longlong * (6 * n) for n in range(_ROW_TENSORS + 1)]
 
 
 def _rows_of(tensors, what: str):
-    """Addresses, sizes and strides of [entries, rows, ...] tensors as the kernels that move rows take them: [(numbers, tensors), ..] a launch."""
-    numbers, spans = [], []
+    """Addresses, sizes and strides of [entries, rows, ...] tensors as the kernels that move rows take them: [(numbers, tensors, kinds), ..] for each call,
+    kinds: 1 rows that lie on 16 bytes, 2 others, 3 both."""
+    calls, numbers, spans, kinds = [], [], [], 0
     for t in tensors:
         shape, stride = t.shape, t.stride()
         if len(shape) < 2:
@@ -1080,15 +1081,20 @@ def _rows_of(tensors, what: str):
                 and not ((E == 1 or outer >= row) and (N == 1 or step >= outer * (E - 1) + row)):
             raise KernelError(f"{what}: rows of a tensor overlap")
         size, base = t.element_size(), t.data_ptr()
-        numbers += (base, E, N, outer * size, step * size, row * size)
         spans.append((base, base + (outer * (E - 1) + step * (N - 1) + row) * size))
+        outer, step, row = outer * size, step * size, row * size
+        numbers += (base, E, N, outer, step, row)
+        kinds |= 2 if (base | outer | step | row) & 15 else 1
+        if len(numbers) == 6 * _ROW_TENSORS:
+            calls.append((_ROW_NUMBERS[_ROW_TENSORS](*numbers), _ROW_TENSORS, kinds))
+            numbers, kinds = [], 0
     if len(spans) > 1:
         spans.sort()
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise KernelError(f"{what}: tensors overlap or lie inside one another")
-    most = 6 * _ROW_TENSORS
-    return [(_ROW_NUMBERS[len(numbers[i:i + most]) // 6](*numbers[i:i + most]), len(numbers[i:i + most]) // 6)
-            for i in range(0, len(numbers), most)]
+    if numbers:
+        calls.append((_ROW_NUMBERS[len(numbers) // 6](*numbers), len(numbers) // 6, kinds))
+    return calls
 
 
 _rows_used = False
@@ -1112,14 +1118,14 @@ def copy_pages(tensors, src: torch.Tensor, dst: torch.Tensor):
     if src.dtype != torch.int32 or dst.dtype != torch.int32 or src.dim() != 1 or src.shape != dst.shape or not src.is_contiguous() \
             or not dst.is_contiguous():
         raise KernelError("copy_pages: src and dst must be contiguous int32 [n]")
-    parts = _rows_of(tensors, "copy_pages")
+    calls = _rows_of(tensors, "copy_pages")
     _here(src, dst, *tensors)
     n = src.shape[0]
-    if n and parts:
+    if n and calls:
         _rows_used = True
-        for of, count in parts:
+        for of, count, kinds in calls:
             _check(library().pico_copy_rows(ctypes.addressof(of), count, src.data_ptr(), dst.data_ptr(), n, _stream()), "copy_pages")
-            _count(-(-n // 65535))
+            _count((2 if kinds == 3 else 1) * -(-n // 65535))
     return tensors
 
 
@@ -1138,11 +1144,11 @@ def reorder_states(states, slots: torch.Tensor, parents: torch.Tensor):
     G, places = slots.shape
     if not 1 <= places <= BEAM_MAX:
         raise KernelError(f"reorder_states: 1 to {BEAM_MAX} places in a group, got {places}")
-    parts = _rows_of(states, "reorder_states")
+    calls = _rows_of(states, "reorder_states")
     _here(slots, parents, *states)
-    if G and parts:
+    if G and calls:
         _rows_used = True
-        for of, count in parts:
+        for of, count, _ in calls:
             _check(library().pico_reorder_rows(ctypes.addressof(of), count, slots.data_ptr(), parents.data_ptr(), G, places, _stream()), "reorder_states")
             _count(-(-G // 65535))
     return states

@@ -157,7 +157,7 @@ def _random_tensor(shape, dtype, g):
 
 
 ROWS = [((3, 40, 16, 8), torch.float32), ((1, 33, 7, 97), torch.bfloat16), ((2, 40, 5), torch.uint8), ((5, 35, 1), torch.int64), ((2, 36, 129, 128), torch.float32),
-        ((4, 34), torch.float32), ((2, 40, 3), torch.bfloat16)]
+        ((4, 34), torch.float32), ((2, 40, 3), torch.bfloat16), ((3, 40, 37), torch.uint8), ((2, 33, 4099), torch.uint8), ((1, 34, 1001, 3), torch.float32)]
 
 
 def _views(t):
