@@ -102,3 +102,21 @@ def test_command_line_searches(tmp_path, capsys):
     llm = LLM(str(tmp_path), dtype="float32", num_pages=32, max_num_seqs=3)
     outs = llm.beam_search([[5, 17, 3], [9]], BeamParams(beams=3, max_new_tokens=5, length_penalty=0.5, ignore_eos=True))
     assert lines == [f"[{i}] {h.score:.6f} {' '.join(map(str, h.token_ids))}" for i, o in enumerate(outs) for h in o.hypotheses]
+
+
+@pytest.mark.parametrize("ahead", [True, False])
+def test_pages_brought_together_between_steps_change_no_token(ahead):
+    """Also with a step in flight and steps that are replayed: a long request goes on while short ones end below it."""
+    from pico_vllm_b200 import SamplingParams
+    prompts = beam_models.prompts_of("qwen2/b", (30, 41, 7, 25))
+    lengths = (3, 40, 5, 24)
+    llm = beam_models.llm("qwen2/b", DEV, 4, at_once=1, use_cuda_graph=True, async_scheduling=ahead)
+    want = [llm.generate([p], SamplingParams(temperature=0.0, max_new_tokens=n, ignore_eos=True))[0].token_ids for p, n in zip(prompts, lengths)]
+    ids = [llm.submit(p, max_new_tokens=n, temperature=0.0, ignore_eos=True) for p, n in zip(prompts, lengths)]
+    llm.mark_finished()
+    done, copied = {}, 0
+    while not llm.is_done():
+        done.update(llm.step())
+        copied += llm.compact_cache()
+        llm.cache.check()
+    assert copied > 0 and [done[i] for i in ids] == [p + w for p, w in zip(prompts, want)]
