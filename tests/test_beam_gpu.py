@@ -285,3 +285,36 @@ def test_rows_moved_in_a_recorded_call():
         graph.replay()
         t = plain.copy(plain.reorder(t, slots.tolist(), family), [p[0] for p in pairs], [p[1] for p in pairs])
         assert torch.equal(d.cpu(), t)
+
+
+def test_another_device_than_the_current_one_is_refused(monkeypatch):
+    from pico_vllm_b200 import ops
+    from pico_vllm_b200.errors import KernelError
+    i32 = dict(dtype=torch.int32, device=DEV)
+    x, s, t = torch.zeros(4, 8, device=DEV), torch.zeros(1, 4, device=DEV), torch.zeros(2, 3, 4, device=DEV)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in (lambda: ops.beam_select(x, s, 4), lambda: ops.copy_pages([t], torch.zeros(1, **i32), torch.zeros(1, **i32)),
+                 lambda: ops.reorder_states([t], torch.zeros(1, 2, **i32), torch.zeros(1, 2, **i32))):
+        with pytest.raises(KernelError, match="current device"):
+            call()
+
+
+def test_on_a_stream_of_its_own():
+    from pico_vllm_b200 import ops
+    g = torch.Generator().manual_seed(6)
+    t, x = torch.randn(3, 30, 5000, generator=g), torch.randn(8, 20001, generator=g) * 3
+    scores = -torch.rand(2, 4, generator=g)
+    slots, parents = [[3, 9, 1, 20], [5, 6, 7, 8]], [[1, 2, 0, 0], [0, 0, 2, 2]]
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        big = torch.randn(4096, 4096, device=DEV)
+        for _ in range(10):
+            big = (big @ big) * 1e-2                   # what comes before is still under way when the calls are made
+        d, lx = t.to(DEV, non_blocking=True), x.to(DEV, non_blocking=True)
+        i32 = dict(dtype=torch.int32, device=DEV)
+        ops.reorder_states([d], torch.tensor(slots, **i32), torch.tensor(parents, **i32))
+        ops.copy_pages([d], torch.tensor([3, 5], **i32), torch.tensor([11, 12], **i32))
+        got = ops.beam_select(lx, scores.to(DEV), 4, 5)
+    stream.synchronize()
+    assert torch.equal(d.cpu(), plain.copy(plain.reorder(t, slots, parents), [3, 5], [11, 12]))
+    _check(x, scores, 4, 5, got, 2, 4, 20001)
