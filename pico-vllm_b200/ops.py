@@ -1062,6 +1062,8 @@ _ROW_NUMBERS = [ctypes.c_longlong * (6 * n) for n in range(_ROW_TENSORS + 1)]
 def _rows_of(tensors, what: str):
     """Addresses, sizes and strides of [entries, rows, ...] tensors as the kernels that move rows take them: [(numbers, tensors, kinds), ..] for each call,
     kinds: 1 rows that lie on 16 bytes, 2 others, 3 both."""
+    if not isinstance(tensors, (list, tuple)):
+        raise KernelError(f"{what}: a list of tensors [entries, rows, ...], got {type(tensors).__name__}")
     calls, numbers, spans, kinds = [], [], [], 0
     for t in tensors:
         shape, stride = t.shape, t.stride()

@@ -34,6 +34,8 @@ def test_choice_refuses(logits, scores, beams, end, out, match):
 
 
 ROWS = [
+    (torch.zeros(2, 3, 4), "a list of tensors"),          # (a list of its entries would be something else)
+    ((t for t in [torch.zeros(2, 3, 4)]), "a list of tensors"),
     ([torch.zeros(5)], "entries, rows"),
     ([torch.zeros(2, 3, 4, 5).transpose(2, 3)], "in one piece"),
     ([torch.zeros(2, 3, 4)[:, :, ::2]], "in one piece"),
