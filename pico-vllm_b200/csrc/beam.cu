@@ -11,8 +11,11 @@
 #define BEAM_THREADS 256
 #define BEAM_LOADS 4                                            // 16-byte loads of a thread under way
 #define BEAM_TILE (BEAM_THREADS * 4 * BEAM_LOADS)               // elements that a block takes at a time
+#define BEAM_AGAIN 2                                            // ... and of the second look
 #define BEAM_MAX 32                                             // beams of a request: lanes of the warp that ranks
 #define BEAM_LIST (4 * BEAM_THREADS + 128)                      // candidates that wait in shared memory (see beam_rows_kernel)
+
+#define BEAM_FEW 6                                              // parts of a row whose lists are merged by searching
 
 typedef unsigned long long u64;
 
@@ -59,10 +62,11 @@ __device__ __forceinline__ u64 beam_mul2(u64 a, u64 b) {
 // Grid (parts, rows).  Block (p, r) reads elements [p * per, (p + 1) * per) of row r (per: a multiple of the tile) and leaves their largest, the sum of
 // exp(x - largest) and their K best, in order.
 // One pass over the elements keeps, in every thread, the running maximum and sum and the maximum of each of its four columns (the 16-byte loads at
-// one place of all tiles); no thread waits for another.  The K-th largest of `groups` >= 4 K maxima of threads then bounds the K-th best from
+// one place of all tiles); no thread waits for another.  The K-th largest of `groups` >= 2 K maxima of threads then bounds the K-th best from
 // below, and only the columns that reach it, a few more than K of 1,024, are read once more (from L2) for the elements themselves.
-// VEC: rows start on 16 bytes; without it the same elements go to the same threads, so that rows of equal numbers have equal sums wherever
-// they lie.
+// VEC: rows start on 16 bytes; otherwise whole words of 16 bytes are read all the same, two for four elements of a thread that lie across them (the second is the
+// neighbour's first, and only words with elements of the row are read).  The same elements go to the same threads either way, so that rows of equal
+// numbers have equal sums wherever they lie.  504 rows of 50,512 that start anywhere: @ us; loads of 4 bytes of four neighbours 26, side by side 30.
 template <bool VEC>
 __global__ void __launch_bounds__(BEAM_THREADS, 6)
 beam_rows_kernel(const float* __restrict__ logits, long long row_stride, int V, int K, int groups, int per, u64* __restrict__ best,
@@ -85,13 +89,20 @@ beam_rows_kernel(const float* __restrict__ logits, long long row_stride, int V, 
     float m = -INFINITY, s = 0.f, column[BEAM_LOADS];
 #pragma unroll
     for (int u = 0; u < BEAM_LOADS; ++u) column[u] = -INFINITY;
+    const int ahead = VEC ? 0 : (int)((uintptr_t)x >> 2) & 3;       // elements of the row's first word of 16 bytes that are not the row's
     auto fetch = [&](float* v, int t0) {
-        if (t0 >= p1) return;
-        if (VEC && t0 + BEAM_TILE <= p1) {
+        if (t0 + BEAM_TILE <= p1) {
 #pragma unroll
             for (int u = 0; u < BEAM_LOADS; ++u) {
-                const float4 q = __ldg(reinterpret_cast<const float4*>(x + t0 + (u * BEAM_THREADS + tid) * 4));
-                v[4 * u] = q.x; v[4 * u + 1] = q.y; v[4 * u + 2] = q.z; v[4 * u + 3] = q.w;
+                const float4* q = reinterpret_cast<const float4*>(x - ahead + t0 + (u * BEAM_THREADS + tid) * 4);
+                const float4 lo = __ldg(q);
+                v[4 * u] = lo.x; v[4 * u + 1] = lo.y; v[4 * u + 2] = lo.z; v[4 * u + 3] = lo.w;
+                if (!VEC && ahead) {
+                    const float4 hi = __ldg(q + 1);
+                    const bool two = ahead & 2, one = ahead & 1;
+                    const float a = two ? lo.z : lo.x, b = two ? lo.w : lo.y, c = two ? hi.x : lo.z, d = two ? hi.y : lo.w, f = two ? hi.z : hi.x;
+                    v[4 * u] = one ? b : a; v[4 * u + 1] = one ? c : b; v[4 * u + 2] = one ? d : c; v[4 * u + 3] = one ? f : d;
+                }
             }
         } else {
 #pragma unroll
@@ -170,33 +181,42 @@ beam_rows_kernel(const float* __restrict__ logits, long long row_stride, int V, 
         }
         __syncthreads();
     };
-    for (int l0 = 0; l0 < loads; l0 += BEAM_THREADS) {
-        const int l = l0 + tid;
-        if (l < loads) {
-            const int c = l / tiles, i = p0 + (l - c * tiles) * BEAM_TILE + columns[c] * 4;
-            float v[4];
-            if (VEC && i + 4 <= p1) {
-                const float4 q = __ldg(reinterpret_cast<const float4*>(x + i));
-                v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    for (int l0 = 0; l0 < loads; l0 += BEAM_AGAIN * BEAM_THREADS) {
+        float v[BEAM_AGAIN][4];
+        int at[BEAM_AGAIN];
+#pragma unroll
+        for (int j = 0; j < BEAM_AGAIN; ++j) {
+            const int l = l0 + j * BEAM_THREADS + tid, c = l / tiles;
+            at[j] = l < loads ? p0 + (l - c * tiles) * BEAM_TILE + columns[c] * 4 : p1;
+            if (VEC && at[j] + 4 <= p1) {
+                const float4 q = __ldg(reinterpret_cast<const float4*>(x + at[j]));
+                v[j][0] = q.x; v[j][1] = q.y; v[j][2] = q.z; v[j][3] = q.w;
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = i + e < p1 ? __ldg(x + i + e) : -INFINITY;
+                for (int e = 0; e < 4; ++e) v[j][e] = at[j] + e < p1 ? __ldg(x + at[j] + e) : -INFINITY;
             }
+        }
+#pragma unroll
+        for (int j = 0; j < BEAM_AGAIN; ++j) {
+            const int done = l0 + (j + 1) * BEAM_THREADS;
+            if (done - BEAM_THREADS >= loads) break;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (v[e] >= bound && v[e] > -INFINITY) {
-                    const u64 key = beam_key(v[e], i + e);
+                if (v[j][e] >= bound && v[j][e] > -INFINITY) {
+                    const u64 key = beam_key(v[j][e], at[j] + e);
                     if (key > least) list[atomicAdd(&s_n, 1)] = key;
                 }
-        }
-        __syncthreads();
-        const int n = s_n;
-        if (l0 + BEAM_THREADS < loads && n > BEAM_LIST - 4 * BEAM_THREADS) {
-            rank(n);
-            if (tid < K) list[tid] = sorted[tid];
-            if (tid == 0) s_n = K;
-            least = sorted[K - 1];
             __syncthreads();
+            const int n = s_n;
+            if (done < loads && n > BEAM_LIST - 4 * BEAM_THREADS) {
+                rank(n);
+                if (tid < K) list[tid] = sorted[tid];
+                if (tid == 0) s_n = K;
+                least = sorted[K - 1];
+                __syncthreads();
+            } else if (done < loads) {
+                __syncthreads();            // all have read the number of candidates
+            }
         }
     }
     rank(s_n);
@@ -224,7 +244,8 @@ __device__ __forceinline__ u64 beam_order(double v) {
 }
 __device__ __forceinline__ double beam_unorder(u64 o) { return __longlong_as_double((long long)(o >> 63 ? o & 0x7fffffffffffffffull : ~o)); }
 
-// Grid (groups), a warp for each of the group's rows.  Warp b merges the lists of row b's parts, a lane for each, then the first warp ranks the rows'
+// Grid (groups), a warp for each of the group's rows.  Warp b merges the lists of row b's parts, a lane for each (few parts: by searching, 64 beams of
+// one part in all @ us less), then the first warp ranks the rows'
 // lists against one another, a lane for each row, until B candidates that go on are found.  What a round waits for are the two warp-wide
 // maxima and the winner's next number, which is there already.  The kernel is all latency, of its instructions too: it is kept short.
 __global__ void beam_join_kernel(const u64* __restrict__ best, const float2* __restrict__ sums, int parts, int K, int rows, int beams, int end_token,
@@ -256,17 +277,41 @@ __global__ void beam_join_kernel(const u64* __restrict__ best, const float2* __r
         const bool dead = !(sum > 0.f && sum < INFINITY) || !isfinite(score);
         asm volatile("cp.async.wait_all;\n" ::: "memory");
         __syncwarp();
-        const u64* q = mine + lane * K;
-        int k = 0;
-        u64 head = lane < parts && !dead ? q[0] : 0ull, next = lane < parts && !dead && K > 1 ? q[1] : 0ull;
+        if (parts <= BEAM_FEW || dead) {
+            // few lists: where each key comes, its own place and how many of the other lists' are larger
+            for (int j = lane; j < K; j += 32) values[b][j] = 0ull;
+            __syncwarp();
 #pragma unroll 1
-        for (int j = 0; j < K; ++j) {
-            const u64 w = beam_warp_max(head);
-            if (lane == 0) values[b][j] = w;
-            if (w != 0ull && head == w) {
-                head = next;
-                ++k;
-                next = k + 1 < K ? q[k + 1] : 0ull;
+            for (int i = lane; i < (dead ? 0 : parts * K); i += 32) {
+                const int p = i / K;
+                const u64 key = mine[i];
+                int at = i - p * K;
+#pragma unroll 1
+                for (int o = 0; o < parts; ++o) {
+                    if (o == p) continue;
+                    int lo = 0, hi = K;
+                    while (lo < hi) {
+                        const int mid = (lo + hi) >> 1;
+                        if (mine[o * K + mid] > key) lo = mid + 1;
+                        else hi = mid;
+                    }
+                    at += lo;
+                }
+                if (key && at < K) values[b][at] = key;
+            }
+        } else {
+            const u64* q = mine + lane * K;
+            int k = 0;
+            u64 head = lane < parts ? q[0] : 0ull, next = lane < parts && K > 1 ? q[1] : 0ull;
+#pragma unroll 1
+            for (int j = 0; j < K; ++j) {
+                const u64 w = beam_warp_max(head);
+                if (lane == 0) values[b][j] = w;
+                if (w != 0ull && head == w) {
+                    head = next;
+                    ++k;
+                    next = k + 1 < K ? q[k + 1] : 0ull;
+                }
             }
         }
         if (lane == 0) ends[b] = -1;
@@ -351,12 +396,12 @@ static int beam_parts(int groups, int rows, int V, int K, long long lists) {
 PICO_API int pico_beam_select(const float* logits, long long row_stride, int groups, int rows, int V, int beams, int end_token, const float* scores,
                               void* scratch, int lists, int* tokens, int* parents, float* out_scores, float* ended, cudaStream_t stream) {
     if (groups < 1 || rows < 1 || rows > beams || beams > BEAM_MAX || V < 1 || (long long)groups * rows > 65535 ||
-        (long long)rows * V > 0x7fffffffll || lists < groups * rows)
+        (long long)rows * V > 0x7ff00000ll || lists < groups * rows)
         return PICO_ERR_SIZE;
     const int K = end_token >= 0 ? 2 * beams : beams, R = groups * rows, parts = beam_parts(groups, rows, V, K, lists);
     const int tiles = (V + BEAM_TILE - 1) / BEAM_TILE, per = (tiles + parts - 1) / parts * BEAM_TILE;
     int sets = 32;
-    while (sets < 4 * K && sets < BEAM_THREADS) sets *= 2;
+    while (sets < 2 * K) sets *= 2;
     u64* best = reinterpret_cast<u64*>(scratch);
     float2* sums = reinterpret_cast<float2*>(best + (size_t)R * parts * K);
     const bool vec = row_stride % 4 == 0 && ((uintptr_t)logits & 15) == 0;

@@ -1044,7 +1044,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, end_toke
              floats.as_strided((G, beams), (beams, 1), at + 2 * c), floats.as_strided((G, rows), (rows, 1), at + 3 * c))
     if G == 0:
         return found
-    if R > 65535 or rows * V > 0x7fffffff:
+    if R > 65535 or rows * V > 0x7FF00000:
         raise KernelError(f"beam_select: {G} requests of {rows} rows with {V} logits are more than the kernel takes")
     lists = max(R, 960)
     scratch = torch.empty(lists * (beams if end_token is None else 2 * beams) + lists, dtype=torch.int64, device=logits.device)

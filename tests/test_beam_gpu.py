@@ -64,7 +64,7 @@ def _check(logits, scores, beams, end, got, G, rows, V):
 
 
 SIZES = [(1, 1, 1, 1), (1, 1, 4, 2), (2, 3, 3, 5), (3, 4, 4, 257), (2, 1, 8, 4096), (5, 2, 5, 4097), (1, 4, 4, 151936), (2, 32, 32, 9001),
-         (1, 32, 32, 20000), (40, 4, 4, 33001), (1, 1, 32, 70000), (3, 7, 19, 12289)]
+         (1, 32, 32, 20000), (2, 20, 20, 30001), (1, 2, 32, 30000), (40, 4, 4, 33001), (1, 1, 32, 70000), (3, 7, 19, 12289)]
 
 
 @pytest.mark.parametrize("G,rows,beams,V", SIZES)
@@ -85,7 +85,7 @@ def test_choice_of_beams(G, rows, beams, V, kind):
     for end in (None, V // 2, int(logits[0].nan_to_num(-math.inf).argmax())):
         got = ops.beam_select(logits, scores, beams, end)
         _check(logits, scores, beams, end, got, G, rows, V)
-        for a, b in zip(got, ops.beam_select(wide[:, 1:1 + V], scores, beams, end)):      # loads of 4 bytes: the same sums
+        for a, b in zip(got, ops.beam_select(wide[:, 1:1 + V], scores, beams, end)):      # rows that start on any 4 bytes: the same sums
             assert torch.equal(a, b)
     ops.check_kernel_status()
 
@@ -318,3 +318,29 @@ def test_on_a_stream_of_its_own():
     stream.synchronize()
     assert torch.equal(d.cpu(), plain.copy(plain.reorder(t, slots, parents), [3, 5], [11, 12]))
     _check(x, scores, 4, 5, got, 2, 4, 20001)
+
+
+def test_a_vocabulary_of_many_millions():
+    """Offsets of bytes beyond 32 bits, and as many parts of a row as the join takes."""
+    from pico_vllm_b200 import ops
+    V = 150_000_003
+    logits = torch.empty(8, V, device=DEV)[6:]             # (starts 3.6 GB into its memory)
+    g = torch.Generator(device=DEV).manual_seed(12)
+    logits.copy_(torch.randint(-30, 0, (2, V), generator=g, device=DEV))
+    at = torch.randperm(V, generator=torch.Generator().manual_seed(1))[:9].tolist()
+    for k, t in enumerate(at):
+        logits[k % 2, t] = 20.0 + 0.25 * k
+    scores = torch.tensor([[-1.0, -0.5]], device=DEV)
+    got = ops.beam_select(logits, scores, 4, at[5])
+    # what the two rows' sums are does not matter to the order here: the large ones differ by 0.25 and more, and so do the normalisers
+    x = logits.double()
+    lse = (x - x.amax(1, keepdim=True)).exp().sum(1).log() + x.amax(1)
+    value = sorted(((20.0 + 0.25 * k - float(lse[k % 2]) + float(scores[0, k % 2]), k % 2, t) for k, t in enumerate(at)), reverse=True)
+    assert all(a[0] - b[0] > 1e-3 for a, b in zip(value, value[1:]))
+    want = [v for v in value if v[2] != at[5]][:4]
+    tokens, parents, new, ended = (t.cpu() for t in got)
+    assert sorted(zip(parents[0].tolist(), tokens[0].tolist())) == sorted((b, t) for _, b, t in want)
+    # sums of up to 1.5e8 / (32 * 256 * 16) tiles of 16 terms a thread, 2^-24 of the sum for each at most
+    for b, t, v in zip(parents[0].tolist(), tokens[0].tolist(), new[0].tolist()):
+        assert abs(v - next(w[0] for w in want if w[1:] == (b, t))) <= (1200 + 64) * 2.0 ** -24 + 2.0 ** -17
+    assert (ended[0, 1] > -math.inf) == ((at[5]) in [v[2] for v in value[:4]]) and ended[0, 0] == -math.inf
