@@ -15,8 +15,6 @@
 #define BEAM_MAX 32                                             // beams of a request: lanes of the warp that ranks
 #define BEAM_LIST (4 * BEAM_THREADS + 128)                      // candidates that wait in shared memory (see beam_rows_kernel)
 
-#define BEAM_FEW 6                                              // parts of a row whose lists are merged by searching
-
 typedef unsigned long long u64;
 
 // A logit and its place as one whole number that is ordered as (logit, earlier place); 0 is below all of them.  -0 counts as 0.
@@ -230,13 +228,6 @@ beam_rows_kernel(const float* __restrict__ logits, long long row_stride, int V, 
     }
 }
 
-// The largest of a warp's 64-bit numbers, in every lane.
-__device__ __forceinline__ u64 beam_warp_max(u64 v) {
-    const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32));
-    const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32) == hi ? (unsigned)v : 0u);
-    return ((u64)hi << 32) | lo;
-}
-
 // A finite number as a whole one that is ordered as it and above 0 (-0 counts as 0), and back.
 __device__ __forceinline__ u64 beam_order(double v) {
     const u64 bits = (u64)__double_as_longlong(v + 0.0);
@@ -244,69 +235,78 @@ __device__ __forceinline__ u64 beam_order(double v) {
 }
 __device__ __forceinline__ double beam_unorder(u64 o) { return __longlong_as_double((long long)(o >> 63 ? o & 0x7fffffffffffffffull : ~o)); }
 
-// Grid (groups), a warp for each of the group's rows.  Warp b merges the lists of row b's parts, a lane for each (few parts: by searching, 64 beams of
-// one part in all @ us less), then the first warp ranks the rows'
-// lists against one another, a lane for each row, until B candidates that go on are found.  What a round waits for are the two warp-wide
-// maxima and the winner's next number, which is there already.  The kernel is all latency, of its instructions too: it is kept short.
-__global__ void beam_join_kernel(const u64* __restrict__ best, const float2* __restrict__ sums, int parts, int K, int rows, int beams, int end_token,
-                                 const float* scores, int* tokens, int* parents, float* out_scores, float* ended) {
+// How many of the K numbers of a falling list are larger than x.
+__device__ __forceinline__ int beam_count(const u64* list, int K, u64 x) {
+    int lo = 0, hi = K;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (list[mid] > x) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+// The largest of a warp's 64-bit numbers, in every lane.
+__device__ __forceinline__ u64 beam_warp_max(u64 v) {
+    const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32));
+    const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32) == hi ? (unsigned)v : 0u);
+    return ((u64)hi << 32) | lo;
+}
+
+// Grid (groups).  First the lists of each row's parts become one: with many parts and few candidates (`rounds`) a warp takes a row, a lane each list, and the
+// largest head is taken K times; else two neighbours at a time are merged, every key finding its place by searching the other list, so that a level
+// costs a few dependent loads however long the lists are.  Then the first warp ranks the rows' lists against one another, a lane for each row,
+// until B candidates that go on are found.  What a round waits for are the two warp-wide maxima and the winner's next number, which is there
+// already.  The kernel is all latency, of its instructions too: it is kept short.
+__global__ void __launch_bounds__(1024) beam_join_kernel(const u64* __restrict__ best, const float2* __restrict__ sums, int parts, int K, int V, int rows,
+                                                         int beams, int end_token, bool rounds, const float* scores, int* tokens, int* parents,
+                                                         float* out_scores, float* ended) {
     pdl_launch_dependents();
-    __shared__ u64 values[BEAM_MAX][2 * BEAM_MAX];              // of the rows' best, in order
-    __shared__ int places[BEAM_MAX][2 * BEAM_MAX];              // their tokens
-    __shared__ int ends[BEAM_MAX];                              // which of them is the end token
-    extern __shared__ __align__(16) u64 beam_keys[];            // [rows][parts][K]
-    const int g = blockIdx.x, lane = threadIdx.x & 31, b = threadIdx.x >> 5;
+    __shared__ double offsets[BEAM_MAX], tops[BEAM_MAX];
+    __shared__ int ends[BEAM_MAX];                              // which of a row's candidates is the end token
+    extern __shared__ __align__(16) u64 beam_keys[];            // [rows * parts][K], and as many lists as half of the parts make
+    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+    const int n = rows * parts * K;
+    u64 *from = beam_keys, *to = from + n;
     pdl_wait();
     {
-        const size_t row = (size_t)g * rows + b;
-        u64* mine = beam_keys + (size_t)b * parts * K;
-        const unsigned to = (unsigned)__cvta_generic_to_shared(mine);
+        const unsigned place = (unsigned)__cvta_generic_to_shared(from);
+        const u64* source = best + (size_t)g * n;
 #pragma unroll 1
-        for (int i = lane; i < parts * K; i += 32)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to + 8u * i), "l"(best + row * parts * K + i) : "memory");
+        for (int i = tid; i < n; i += blockDim.x)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(place + 8u * i), "l"(source + i) : "memory");
+    }
+#pragma unroll 1
+    for (int b = tid >> 5; b < rows; b += blockDim.x >> 5) {
+        const size_t row = (size_t)g * rows + b;
         const float2 c = lane < parts ? sums[row * parts + lane] : make_float2(-INFINITY, 0.f);
         const float score = scores[row];
         const float top = warp_max(c.x);
         const float sum = warp_sum(c.x == -INFINITY ? c.y : c.y * beam_exp2((c.x - top) * 1.4426950408889634f));
-        // log(f * 2^n), f in [1, 2): the whole part in 64 bits, so that the result is off by the rounding of a number below 0.7
-        const int n = (int)(__float_as_uint(sum) >> 23) - 127;
+        // log(f * 2^e), f in [1, 2): the whole part in 64 bits, so that the result is off by the rounding of a number below 0.7
+        const int e = (int)(__float_as_uint(sum) >> 23) - 127;
         const float f = __uint_as_float((__float_as_uint(sum) & 0x007fffffu) | 0x3f800000u);
-        // v = (x - largest) + (s - log sum): as near to s as it gets, however large the logits are
-        const double off = (double)score - ((double)n * 0.69314718055994530942 + (double)logf(f));
         // (a row with an infinity or without any number: its sum is none or 0)
         const bool dead = !(sum > 0.f && sum < INFINITY) || !isfinite(score);
-        asm volatile("cp.async.wait_all;\n" ::: "memory");
-        __syncwarp();
-        if (parts <= BEAM_FEW || dead) {
-            // few lists: where each key comes, its own place and how many of the other lists' are larger
-            for (int j = lane; j < K; j += 32) values[b][j] = 0ull;
-            __syncwarp();
+        if (lane == 0) {
+            // v = (x - largest) + (s - log sum): as near to s as it gets, however large the logits are
+            offsets[b] = dead ? INFINITY : (double)score - ((double)e * 0.69314718055994530942 + (double)logf(f));
+            tops[b] = (double)top;
+            ends[b] = -1;
+        }
+    }
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+    __syncthreads();
+    int lists = parts;                  // of a row
+    if (rounds) {
 #pragma unroll 1
-            for (int i = lane; i < (dead ? 0 : parts * K); i += 32) {
-                const int p = i / K;
-                const u64 key = mine[i];
-                int at = i - p * K;
-#pragma unroll 1
-                for (int o = 0; o < parts; ++o) {
-                    if (o == p) continue;
-                    int lo = 0, hi = K;
-                    while (lo < hi) {
-                        const int mid = (lo + hi) >> 1;
-                        if (mine[o * K + mid] > key) lo = mid + 1;
-                        else hi = mid;
-                    }
-                    at += lo;
-                }
-                if (key && at < K) values[b][at] = key;
-            }
-        } else {
-            const u64* q = mine + lane * K;
+        for (int b = tid >> 5; b < rows; b += blockDim.x >> 5) {
+            const u64* q = from + (b * parts + lane) * K;
             int k = 0;
             u64 head = lane < parts ? q[0] : 0ull, next = lane < parts && K > 1 ? q[1] : 0ull;
 #pragma unroll 1
             for (int j = 0; j < K; ++j) {
                 const u64 w = beam_warp_max(head);
-                if (lane == 0) values[b][j] = w;
+                if (lane == 0) to[b * K + j] = w;
                 if (w != 0ull && head == w) {
                     head = next;
                     ++k;
@@ -314,38 +314,63 @@ __global__ void beam_join_kernel(const u64* __restrict__ best, const float2* __r
                 }
             }
         }
-        if (lane == 0) ends[b] = -1;
-        __syncwarp();
+        from = to;
+        __syncthreads();
+    } else {
 #pragma unroll 1
-        for (int j = lane; j < K; j += 32) {
-            const u64 key = values[b][j];
-            const int t = beam_key_at(key);
-            values[b][j] = key ? beam_order(((double)beam_key_logit(key) - (double)top) + off) : 0ull;
-            places[b][j] = t;
-            if (key && t == end_token) ends[b] = j;
+        while (lists > 1) {
+            const int left = (lists + 1) >> 1;
+#pragma unroll 1
+            for (int i = tid; i < rows * lists * K; i += blockDim.x) {
+                const int l = i / K, b = l / lists, p = l - b * lists, other = p ^ 1;
+                const u64 x = from[i];
+                int at = i - l * K;
+                if (other < lists) at += beam_count(from + (l - p + other) * K, K, x);
+                // (of empty places, which are equal, the odd list's come behind)
+                if (x == 0ull && (p & 1)) at = K;
+                if (at < K) to[(b * left + (p >> 1)) * K + at] = x;
+            }
+            __syncthreads();
+            u64* const v = from;
+            from = to;
+            to = v;
+            lists = left;
         }
     }
+    // ---- keys become values, their tokens beside them
+    int* const at = reinterpret_cast<int*>(beam_keys + n + (size_t)rows * ((parts + 1) / 2) * K);
+#pragma unroll 1
+    for (int i = tid; i < rows * K; i += blockDim.x) {
+        const int b = i / K;
+        const u64 key = from[i];
+        const double off = offsets[b];
+        from[i] = key && off < INFINITY ? beam_order(((double)beam_key_logit(key) - tops[b]) + off) : 0ull;
+        at[i] = beam_key_at(key);
+        if (key && beam_key_at(key) == end_token) ends[b] = i - b * K;
+    }
     __syncthreads();
-    if (b != 0) return;
-    const u64* list = values[lane < rows ? lane : 0];
+    if (tid >= 32) return;
+    const int row = lane < rows ? lane : 0;
+    const u64* list = from + row * K;
     const int end_at = lane < rows ? ends[lane] : -1;
     int k = 0;
     u64 value = lane < rows ? list[0] : 0ull, next = lane < rows && K > 1 ? list[1] : 0ull;
     int my_parent = -1, my_k = 0, end_k = -1, count = 0;
     unsigned has = 0u;                  // parents with a child
     bool extra = lane < beams;
+#pragma unroll 1
     for (int rank = 0; count < beams && rank < K; ++rank) {
         const u64 w = beam_warp_max(value);
         if (w == 0ull) break;
         const int who = __ffs(__ballot_sync(0xffffffffu, value == w)) - 1;        // of equal ones the first beam
         const bool won = lane == who;
-        const int at = __shfl_sync(0xffffffffu, k, who);
+        const int which = __shfl_sync(0xffffffffu, k, who);
         if (__any_sync(0xffffffffu, won && k == end_at)) {
             if (won && rank < beams) end_k = k;
         } else {
             if (lane == count) {
                 my_parent = who;
-                my_k = at;
+                my_k = which;
                 extra = (has >> who) & 1u;
             }
             has |= 1u << who;
@@ -366,15 +391,15 @@ __global__ void beam_join_kernel(const u64* __restrict__ best, const float2* __r
             for (int e = __popc(others & ((1u << lane) - 1u)); e > 0; --e) left &= left - 1u;
             place = __ffs(left) - 1;
         }
-        const int at = g * beams + place;
-        tokens[at] = my_parent < 0 ? -1 : places[my_parent][my_k];
-        parents[at] = my_parent < 0 ? place : my_parent;
-        out_scores[at] = my_parent < 0 ? -INFINITY : (float)beam_unorder(values[my_parent][my_k]);
+        const int o = g * beams + place;
+        tokens[o] = my_parent < 0 ? -1 : at[my_parent * K + my_k];
+        parents[o] = my_parent < 0 ? place : my_parent;
+        out_scores[o] = my_parent < 0 ? -INFINITY : (float)beam_unorder(from[my_parent * K + my_k]);
     }
     if (lane < rows) ended[g * rows + lane] = end_k < 0 ? -INFINITY : (float)beam_unorder(list[end_k]);
 }
 
-#define BEAM_JOIN_KEYS 20480    // candidates that a block of beam_join_kernel has room for in shared memory (160 KB)
+#define BEAM_JOIN_KEYS 8192     // candidates that a block of beam_join_kernel has room for in shared memory (up to 136 KB)
 
 // Parts of a row: as many as run at once over all rows (256 rows of 151,936 in 1 / 2 / 3 / 4 / 7 parts: 44 / 43 / 35 / 42 / 36 us with the join; four rows in
 // 7 / 10 / 19: 8.9 / 8.3 / 7.6), none shorter than a tile, and no more than the join (a lane each) and the scratch have room for.
@@ -405,15 +430,23 @@ PICO_API int pico_beam_select(const float* logits, long long row_stride, int gro
     u64* best = reinterpret_cast<u64*>(scratch);
     float2* sums = reinterpret_cast<float2*>(best + (size_t)R * parts * K);
     const bool vec = row_stride % 4 == 0 && ((uintptr_t)logits & 15) == 0;
-    const size_t smem = (size_t)rows * parts * K * sizeof(u64);
-    if (smem > 20 * 1024) {             // beside the kernel's own 25 KB
+    const int n = rows * parts * K;
+    const size_t smem = (size_t)(n + rows * ((parts + 1) / 2) * K) * sizeof(u64) + (size_t)rows * K * sizeof(int);
+    if (smem > 40 * 1024) {             // beside the kernel's own
         const cudaError_t e = cudaFuncSetAttribute(beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)cudaGetLastError();
     }
+    // a round takes some 100 cycles, a level of merging 350
+    int levels = 0;
+    while ((1 << levels) < parts) ++levels;
+    const bool rounds = 2 * K < 7 * levels;
+    int threads = ((rounds ? rows * K : n) / 2 + 31) / 32 * 32;
+    threads = threads < 128 ? 128 : threads;
+    threads = threads < 32 * rows ? 32 * rows : threads > 1024 ? 1024 : threads;
     pico_launch(vec ? beam_rows_kernel<true> : beam_rows_kernel<false>, dim3(parts, R), dim3(BEAM_THREADS), 0, stream, logits, row_stride, V, K, sets, per, best, sums);
     const int status = pico_launch_status();
     if (status) return status;
-    pico_launch(beam_join_kernel, dim3(groups), dim3(32 * rows), smem, stream, (const u64*)best, (const float2*)sums, parts, K, rows, beams, end_token,
-                scores, tokens, parents, out_scores, ended);
+    pico_launch(beam_join_kernel, dim3(groups), dim3(threads), smem, stream, (const u64*)best, (const float2*)sums, parts, K, V, rows, beams, end_token,
+                rounds, scores, tokens, parents, out_scores, ended);
     return pico_launch_status();
 }
