@@ -64,7 +64,7 @@ __device__ __forceinline__ u64 beam_mul2(u64 a, u64 b) {
 // below, and only the columns that reach it, a few more than K of 1,024, are read once more (from L2) for the elements themselves.
 // VEC: rows start on 16 bytes; otherwise whole words of 16 bytes are read all the same, two for four elements of a thread that lie across them (the second is the
 // neighbour's first, and only words with elements of the row are read).  The same elements go to the same threads either way, so that rows of equal
-// numbers have equal sums wherever they lie.  504 rows of 50,512 that start anywhere: @ us; loads of 4 bytes of four neighbours 26, side by side 30.
+// numbers have equal sums wherever they lie.  504 rows of 50,512 that start anywhere take 31.5 us, by loads of 4 bytes 33.7.
 template <bool VEC>
 __global__ void __launch_bounds__(BEAM_THREADS, 6)
 beam_rows_kernel(const float* __restrict__ logits, long long row_stride, int V, int K, int groups, int per, u64* __restrict__ best,
@@ -245,11 +245,18 @@ __device__ __forceinline__ int beam_count(const u64* list, int K, u64 x) {
     }
     return lo;
 }
-// The largest of a warp's 64-bit numbers, in every lane.
-__device__ __forceinline__ u64 beam_warp_max(u64 v) {
-    const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32));
-    const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(v >> 32) == hi ? (unsigned)v : 0u);
-    return ((u64)hi << 32) | lo;
+// The lane with the largest of a warp's 64-bit numbers, of equal ones the first, as a bit; 0: all are 0 (others have higher halves above 0).  Mostly the higher
+// halves tell; the chain of a round is a maximum, a vote and a branch that all lanes take alike (some 80 cycles).
+__device__ __forceinline__ unsigned beam_winner(u64 v) {
+    const unsigned hi = (unsigned)(v >> 32), top = __reduce_max_sync(0xffffffffu, hi);
+    unsigned lanes = __ballot_sync(0xffffffffu, hi == top);
+    if (lanes & (lanes - 1u)) {
+        if (top == 0u) return 0u;
+        const unsigned lo = hi == top ? (unsigned)v : 0u, low = __reduce_max_sync(0xffffffffu, lo);
+        lanes = __ballot_sync(0xffffffffu, hi == top && lo == low);
+        lanes &= 0u - lanes;
+    }
+    return lanes;
 }
 
 // Grid (groups).  First the lists of each row's parts become one: with many parts and few candidates (`rounds`) a warp takes a row, a lane each list, and the
@@ -263,6 +270,7 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const u64* __restrict__
     pdl_launch_dependents();
     __shared__ double offsets[BEAM_MAX], tops[BEAM_MAX];
     __shared__ int ends[BEAM_MAX];                              // which of a row's candidates is the end token
+    __shared__ int taken[2 * BEAM_MAX];                         // which of its row's candidates has a rank
     extern __shared__ __align__(16) u64 beam_keys[];            // [rows * parts][K], and as many lists as half of the parts make
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
     const int n = rows * parts * K;
@@ -305,13 +313,12 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const u64* __restrict__
             u64 head = lane < parts ? q[0] : 0ull, next = lane < parts && K > 1 ? q[1] : 0ull;
 #pragma unroll 1
             for (int j = 0; j < K; ++j) {
-                const u64 w = beam_warp_max(head);
-                if (lane == 0) to[b * K + j] = w;
-                if (w != 0ull && head == w) {
-                    head = next;
-                    ++k;
-                    next = k + 1 < K ? q[k + 1] : 0ull;
-                }
+                const unsigned winner = beam_winner(head);
+                const bool won = (winner >> lane) & 1u;
+                if (won || (winner == 0u && lane == 0)) to[b * K + j] = head;
+                k += won;
+                head = won ? next : head;
+                next = lane < parts && k + 1 < K ? q[k + 1] : 0ull;
             }
         }
         from = to;
@@ -355,33 +362,30 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const u64* __restrict__
     const int end_at = lane < rows ? ends[lane] : -1;
     int k = 0;
     u64 value = lane < rows ? list[0] : 0ull, next = lane < rows && K > 1 ? list[1] : 0ull;
-    int my_parent = -1, my_k = 0, end_k = -1, count = 0;
-    unsigned has = 0u;                  // parents with a child
+    int my_rank = -1, end_k = -1, count = 0;
+    unsigned my_bit = 0u, has = 0u;     // the parent; parents with a child
     bool extra = lane < beams;
 #pragma unroll 1
     for (int rank = 0; count < beams && rank < K; ++rank) {
-        const u64 w = beam_warp_max(value);
-        if (w == 0ull) break;
-        const int who = __ffs(__ballot_sync(0xffffffffu, value == w)) - 1;        // of equal ones the first beam
-        const bool won = lane == who;
-        const int which = __shfl_sync(0xffffffffu, k, who);
-        if (__any_sync(0xffffffffu, won && k == end_at)) {
-            if (won && rank < beams) end_k = k;
-        } else {
-            if (lane == count) {
-                my_parent = who;
-                my_k = which;
-                extra = (has >> who) & 1u;
-            }
-            has |= 1u << who;
-            ++count;
+        const unsigned at_end = __ballot_sync(0xffffffffu, k == end_at);
+        const unsigned winner = beam_winner(value);             // of equal ones the first beam
+        if (winner == 0u) break;
+        const bool won = (winner >> lane) & 1u, ends_here = (at_end & winner) != 0u;
+        if (won) taken[rank] = k;
+        if (won && ends_here && rank < beams) end_k = k;
+        if (lane == count && !ends_here) {
+            my_rank = rank;
+            my_bit = winner;
+            extra = has & winner;
         }
-        if (won) {
-            value = next;
-            ++k;
-            next = k + 1 < K ? list[k + 1] : 0ull;
-        }
+        has |= ends_here ? 0u : winner;
+        count += !ends_here;
+        k += won;
+        value = won ? next : value;
+        next = lane < rows && k + 1 < K ? list[k + 1] : 0ull;
     }
+    __syncwarp();
+    const int my_parent = __ffs(my_bit) - 1, my_k = my_rank < 0 ? 0 : taken[my_rank];
     // places: the first child of a parent has the parent's, the others (and those that hold nothing) the ones that are left
     const unsigned others = __ballot_sync(0xffffffffu, extra);
     if (lane < beams) {
@@ -401,8 +405,8 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const u64* __restrict__
 
 #define BEAM_JOIN_KEYS 8192     // candidates that a block of beam_join_kernel has room for in shared memory (up to 136 KB)
 
-// Parts of a row: as many as run at once over all rows (256 rows of 151,936 in 1 / 2 / 3 / 4 / 7 parts: 44 / 43 / 35 / 42 / 36 us with the join; four rows in
-// 7 / 10 / 19: 8.9 / 8.3 / 7.6), none shorter than a tile, and no more than the join (a lane each) and the scratch have room for.
+// Parts of a row: as many as run at once over all rows (256 rows of 151,936 in 1 / 2 / 3 / 4 / 7 parts: 44 / 43 / 35 / 42 / 36 us with the join of then, now 32 in 3;
+// four rows in 7 / 10 / 19: 8.9 / 8.3 / 7.6), none shorter than a tile, and no more than the join (a lane each) and the scratch have room for.
 static int beam_parts(int groups, int rows, int V, int K, long long lists) {
     const int tiles = (V + BEAM_TILE - 1) / BEAM_TILE, R = groups * rows;
     long long want = (6 * pico_num_sms()) / R;
@@ -436,10 +440,11 @@ PICO_API int pico_beam_select(const float* logits, long long row_stride, int gro
         const cudaError_t e = cudaFuncSetAttribute(beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return (int)cudaGetLastError();
     }
-    // a round takes some 100 cycles, a level of merging 350
-    int levels = 0;
-    while ((1 << levels) < parts) ++levels;
-    const bool rounds = 2 * K < 7 * levels;
+    // a round takes some 100 cycles or more, as many warps as there are rows share the multiprocessor; a level of merging 350, or two a number (16 rows of 8
+    // beams in 19 parts: by rounds 10.7 us, by levels 11.8; two of 28 beams in 16 parts 17.6 and 14.1)
+    int by_rounds = K * (100 > 6 * rows ? 100 : 6 * rows), by_levels = 0;
+    for (int left = parts, m = n; left > 1; left = (left + 1) / 2, m = rows * left * K) by_levels += 2 * m > 350 ? 2 * m : 350;
+    const bool rounds = by_rounds < by_levels;
     int threads = ((rounds ? rows * K : n) / 2 + 31) / 32 * 32;
     threads = threads < 128 ? 128 : threads;
     threads = threads < 32 * rows ? 32 * rows : threads > 1024 ? 1024 : threads;
