@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from array import array
 from typing import Optional
 
 import torch
@@ -988,19 +989,6 @@ def _here(*tensors) -> None:
                 raise KernelError(f"kernel arguments must lie on the current device (cuda:{dev}), got {t.device}")
 
 
-def _span(t: torch.Tensor):
-    """First byte of a tensor and the byte behind its last."""
-    start = t.data_ptr()
-    if t.numel() == 0:
-        return start, start
-    return start, start + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-
-
-def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a1 <= b0 or b1 <= a0
-
-
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, end_token: Optional[int] = None,
                 out: Optional[torch.Tensor] = None):
     """One step of beam search for several requests: which beams go on, with which token, and which hypotheses end.
@@ -1036,8 +1024,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, end_toke
         if out.dtype != torch.int32 or out.shape != (n,) or not out.is_contiguous():
             raise KernelError(f"beam_select: out must be contiguous int32 [{n}]")
         _here(logits, scores, out)
-        same = rows == beams and scores.data_ptr() == out.data_ptr() + 8 * c
-        if not (_apart(logits, out) and (same or _apart(scores, out))):
+        o, x, s = out.data_ptr(), logits.data_ptr(), scores.data_ptr()
+        same = rows == beams and s == o + 8 * c         # the new scores of an earlier call
+        if (x < o + 4 * n and o < x + 4 * ((R - 1) * logits.stride(0) + V)) or (not same and s < o + 4 * n and o < s + 4 * R):
             raise KernelError("beam_select: out overlaps the inputs")
     floats, at = out.view(torch.float32), out.storage_offset()
     found = (out.as_strided((G, beams), (beams, 1), at), out.as_strided((G, beams), (beams, 1), at + c),
@@ -1056,7 +1045,21 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, end_toke
     return found
 
 
-_ROW_NUMBERS = [ctypes.c_longlong * (6 * n) for n in range(_ROW_TENSORS + 1)]
+def _row_strides(t: torch.Tensor, what: str):
+    """(bytes between entries, bytes between rows, bytes of a row) of a tensor [entries, rows, ...] that is not contiguous; refuses what is no such tensor."""
+    shape, stride, size = t.shape, t.stride(), t.element_size()
+    row = 1
+    for n, s in zip(shape[:1:-1], stride[:1:-1]):
+        if s != row and n > 1 and t.numel():
+            raise KernelError(f"{what}: tensors are [entries, rows, ...], each row of an entry in one piece")
+        row *= n
+    E, N = shape[0], shape[1]
+    outer, step = stride[0] if E > 1 else 0, stride[1] if N > 1 else 0
+    # no two rows may share a byte: rows within an entry, entries within a row's place, or one of the two alone
+    if not ((N == 1 or step >= row) and (E == 1 or outer >= step * (N - 1) + row)) \
+            and not ((E == 1 or outer >= row) and (N == 1 or step >= outer * (E - 1) + row)):
+        raise KernelError(f"{what}: rows of a tensor overlap")
+    return outer * size, step * size, row * size
 
 
 def _rows_of(tensors, what: str):
@@ -1066,36 +1069,35 @@ def _rows_of(tensors, what: str):
         raise KernelError(f"{what}: a list of tensors [entries, rows, ...], got {type(tensors).__name__}")
     calls, numbers, spans, kinds = [], [], [], 0
     for t in tensors:
-        shape, stride = t.shape, t.stride()
+        shape = t.shape
         if len(shape) < 2:
             raise KernelError(f"{what}: tensors are [entries, rows, ...], each row of an entry in one piece")
         E, N = shape[0], shape[1]
-        row = 1
-        for n, s in zip(shape[:1:-1], stride[:1:-1]):
-            if s != row and n > 1 and t.numel():
-                raise KernelError(f"{what}: tensors are [entries, rows, ...], each row of an entry in one piece")
-            row *= n
-        if row == 0 or E == 0 or N == 0:
-            continue
-        outer, step = stride[0] if E > 1 else 0, stride[1] if N > 1 else 0
-        # no two rows may share a byte: rows within an entry, entries within a row's place, or one of the two alone
-        if not ((N == 1 or step >= row) and (E == 1 or outer >= step * (N - 1) + row)) \
-                and not ((E == 1 or outer >= row) and (N == 1 or step >= outer * (E - 1) + row)):
-            raise KernelError(f"{what}: rows of a tensor overlap")
-        size, base = t.element_size(), t.data_ptr()
-        spans.append((base, base + (outer * (E - 1) + step * (N - 1) + row) * size))
-        outer, step, row = outer * size, step * size, row * size
+        if t.is_contiguous():
+            size = t.nbytes
+            if size == 0:
+                continue
+            row = step = size // (E * N)
+            outer = row * N
+        else:
+            outer, step, row = _row_strides(t, what)
+            size = outer * (E - 1) + step * (N - 1) + row
+        base = t.data_ptr()
+        spans.append((base, base + size))
         numbers += (base, E, N, outer, step, row)
         kinds |= 2 if (base | outer | step | row) & 15 else 1
         if len(numbers) == 6 * _ROW_TENSORS:
-            calls.append((_ROW_NUMBERS[_ROW_TENSORS](*numbers), _ROW_TENSORS, kinds))
+            calls.append((array("q", numbers), _ROW_TENSORS, kinds))
             numbers, kinds = [], 0
     if len(spans) > 1:
         spans.sort()
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise KernelError(f"{what}: tensors overlap or lie inside one another")
+        end = 0
+        for first, last in spans:
+            if first < end:
+                raise KernelError(f"{what}: tensors overlap or lie inside one another")
+            end = last
     if numbers:
-        calls.append((_ROW_NUMBERS[len(numbers) // 6](*numbers), len(numbers) // 6, kinds))
+        calls.append((array("q", numbers), len(numbers) // 6, kinds))
     return calls
 
 
@@ -1126,7 +1128,7 @@ def copy_pages(tensors, src: torch.Tensor, dst: torch.Tensor):
     if n and calls:
         _rows_used = True
         for of, count, kinds in calls:
-            _check(library().pico_copy_rows(ctypes.addressof(of), count, src.data_ptr(), dst.data_ptr(), n, _stream()), "copy_pages")
+            _check(library().pico_copy_rows(of.buffer_info()[0], count, src.data_ptr(), dst.data_ptr(), n, _stream()), "copy_pages")
             _count((2 if kinds == 3 else 1) * -(-n // 65535))
     return tensors
 
@@ -1151,7 +1153,7 @@ def reorder_states(states, slots: torch.Tensor, parents: torch.Tensor):
     if G and calls:
         _rows_used = True
         for of, count, _ in calls:
-            _check(library().pico_reorder_rows(ctypes.addressof(of), count, slots.data_ptr(), parents.data_ptr(), G, places, _stream()), "reorder_states")
+            _check(library().pico_reorder_rows(of.buffer_info()[0], count, slots.data_ptr(), parents.data_ptr(), G, places, _stream()), "reorder_states")
             _count(-(-G // 65535))
     return states
 

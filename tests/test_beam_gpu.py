@@ -344,3 +344,21 @@ def test_a_vocabulary_of_many_millions():
     for b, t, v in zip(parents[0].tolist(), tokens[0].tolist(), new[0].tolist()):
         assert abs(v - next(w[0] for w in want if w[1:] == (b, t))) <= (1200 + 64) * 2.0 ** -24 + 2.0 ** -17
     assert (ended[0, 1] > -math.inf) == ((at[5]) in [v[2] for v in value[:4]]) and ended[0, 0] == -math.inf
+
+
+def test_a_buffer_that_overlaps_the_inputs_is_refused():
+    from pico_vllm_b200 import ops
+    from pico_vllm_b200.errors import KernelError
+    memory = torch.zeros(4000, dtype=torch.int32, device=DEV)
+    floats = memory.view(torch.float32)
+    logits, scores, out = floats[:800].view(8, 100), floats[900:908].view(2, 4), memory[1000:1032]
+    ops.beam_select(logits, scores, 4, None, out)
+    ops.beam_select(logits, out[16:24].view(torch.float32).view(2, 4), 4, None, out)              # the new scores of before
+    for at in (0, 768, 799, 876, 901, 907):
+        with pytest.raises(KernelError, match="overlaps"):
+            ops.beam_select(logits, scores, 4, None, memory[at:at + 32])
+    ops.beam_select(logits, scores, 4, None, memory[800:832])
+    with pytest.raises(KernelError, match="overlaps"):
+        ops.beam_select(logits, out[15:23].view(torch.float32).view(2, 4), 4, None, out)
+    with pytest.raises(KernelError, match="overlaps"):                                            # two rows for four beams: other places
+        ops.beam_select(logits[:4], out[16:20].view(torch.float32).view(2, 2), 4, None, memory[1000:1028])
