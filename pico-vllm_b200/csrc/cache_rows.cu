@@ -120,6 +120,8 @@ __device__ __forceinline__ void copy_shifted(const RowTensor& t, int block, int 
 }
 
 // Grid (blocks of a row over all tensors, pairs): row dst[y] becomes row src[y].  A pair with a negative index, or of a row with itself, is passed over.
+// Bound by memory: 1,000 pages of 0.9 MB take 280 us (6.5 TB/s, as a plain copy), 128 of 0.46 MB 21 (18 at that rate, and a launch).  16 KB a block, four loads a thread
+// under way, eight blocks to a multiprocessor.
 // SHIFTED: sizes, strides and starts that are no multiples of 16 bytes.  1,201 rows of 9 x 1,358 bytes in pairs of bytes take 16.1 us, so 9.2.
 template <bool SHIFTED>
 __global__ void __launch_bounds__(ROWS_THREADS) copy_rows_kernel(RowTensors ts, const int* __restrict__ src, const int* __restrict__ dst) {

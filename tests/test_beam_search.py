@@ -230,6 +230,23 @@ def test_requests_and_searches_one_after_the_other(on_cpu):
     assert done[long] == prompts[0] + want[0] and done[short] == prompts[1] + want[1][:2] and copied > 0
 
 
+@pytest.mark.parametrize("end_at", [None, 0, 2])
+def test_a_single_token(on_cpu, end_at):
+    """Nothing branches: the choice after the prompt is all, the end token among it or not."""
+    from pico_vllm_b200 import BeamParams
+    prompts = beam_models.prompts_of("qwen2/a", (16, 5))
+    next_logits = beam_models.model("qwen2/a")[3]
+    lp = next_logits(prompts[0]).log_softmax(0).sort(descending=True)
+    end = None if end_at is None else int(lp.indices[end_at])
+    llm = beam_models.llm("qwen2/a", "cpu", 4, end_token=end)
+    outs = llm.beam_search(prompts, BeamParams(beams=4, max_new_tokens=1))
+    compare(outs, prompts, next_logits, 4, 1, end, 1.0, 2e-5)
+    if end is not None:
+        assert [h.finish_reason for h in outs[0].hypotheses] == ["eos" if k == end_at else "length" for k in range(4)]
+    llm.cache.check()
+    assert all(g.pool.in_use == 0 for g in llm.cache.groups)
+
+
 def test_searches_refused(on_cpu):
     from pico_vllm_b200 import BeamParams
     for bad in (dict(beams=0), dict(beams=33), dict(max_new_tokens=0), dict(length_penalty=-1.0), dict(length_penalty=float("nan")),
