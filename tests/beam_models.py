@@ -39,10 +39,14 @@ SEARCHES = [("qwen2/a", (1, 16, 37), 4, 20, 1.0), ("qwen2/b", (8, 30, 5, 24), 3,
 
 
 def llm(name, device, beams, at_once=2, end_token=None, dtype="float32", **options):
+    config, tensors, page, _ = model(name)
+    return llm_of(config, tensors, device, beams, at_once, end_token, dtype, **{"page_size": page, **options})
+
+
+def llm_of(config, tensors, device, beams, at_once=2, end_token=None, dtype="float32", **options):
     from pico_vllm_b200 import LLM, EngineConfig
     from pico_vllm_b200.engine import model_from_tensors
-    config, tensors, page, _ = model(name)
-    options = {"use_cuda_graph": False, "max_cache_tokens": 1024, "max_num_batched_tokens": 16, "page_size": page, **options}
+    options = {"use_cuda_graph": False, "max_cache_tokens": 1024, "max_num_batched_tokens": 16, **options}
     ecfg = EngineConfig(dtype=dtype, device=device, max_num_seqs=at_once * beams, **options)
     m = model_from_tensors(config, tensors, ecfg)
     out = LLM(m, engine_config=ecfg)

@@ -54,6 +54,45 @@ def test_scores_are_those_of_the_tokens_in_bfloat16(name, beams):
             assert abs(total - h.score) <= 2e-2 * most * math.sqrt(len(h.token_ids)), (total, h.score, most)
 
 
+DESIGNS = [(m, k) for m, names in (("zapipel", "pqmr"), ("zikupel", "abcd"), ("zazilix", "abcd"), ("banazen", "abc"), ("vanapel", "abcd"), ("zegorax", "abcd"))
+           for k in names]
+
+
+@pytest.mark.parametrize("design,name", DESIGNS)
+def test_every_design_searches(design, name):
+    """Latents, pages of windows, states of every kind, layers that read another's cache: each hypothesis run again as a request of its own has the score
+    that the search gave it, in 32 bits.  A logit is off by at most 5e-5 of the largest (the designs' own tests), a token's log-probability by twice that; what
+    a beam would take from another one is off by 1e-2 and more."""
+    import importlib
+    from pico_vllm_b200 import BeamParams
+    from pico_vllm_b200.engine import StepItem
+    from pico_vllm_b200.registry import config_from_dict
+    module = importlib.import_module(f"test_{design}_gpu")
+    raw = module.SHAPES[name]
+    tensors = module._tensors(name) if design == "zapipel" else module._tensors(raw, module.SEEDS[name])
+    llm = beam_models.llm_of(config_from_dict(raw), tensors, DEV, 4, page_size=8, use_cuda_graph=True, max_num_batched_tokens=24, max_model_len=64,
+                             max_cache_tokens=640)
+    import helpers
+    prompts = [helpers.random_ids(n, llm.model.vocab_size, 60 + n) for n in (27, 8)]
+    moved, reorder = [], llm.cache.reorder
+    llm.cache.reorder = lambda slots, parents, *more: (moved.extend(q != p for f in parents for p, q in enumerate(f)), reorder(slots, parents, *more))[1]
+    outs = llm.beam_search(prompts, BeamParams(beams=4, max_new_tokens=21, ignore_eos=True))
+    assert sum(moved) >= 4                  # beams died and others branched off
+    for p, o in zip(prompts, outs):
+        assert len({tuple(h.token_ids) for h in o.hypotheses}) == 4
+        for h in o.hypotheses:
+            slot = llm.cache.acquire("again")
+            logits = llm.runner.step([StepItem(slot, p, (len(p) - 1,))])
+            total, most = 0.0, 0.0
+            for k, t in enumerate(h.token_ids):
+                total, most = total + float(logits[0].double().log_softmax(0)[t]), max(most, float(logits[0].abs().max()))
+                if k + 1 < len(h.token_ids):
+                    logits = llm.runner.step([StepItem(slot, [t], (0,))])
+            llm.cache.release(slot)
+            assert abs(total - h.score) <= 1e-4 * most * len(h.token_ids), (total, h.score, most)
+    llm.cache.check()
+
+
 def test_branches_on_the_device():
     """The cache's branches with the kernels: fork, reorder (with the indices here or on the device), compact, and pages of a window."""
     import random
