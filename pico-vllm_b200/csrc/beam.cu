@@ -265,8 +265,7 @@ __device__ __forceinline__ unsigned beam_winner(u64 v) {
 // largest head is taken K times; else two neighbours at a time are merged, every key finding its place by searching the other list, so that a level
 // costs a few dependent loads however long the lists are.  Then the first warp ranks the rows' lists against one another, a lane for each row,
 // until B candidates that go on are found.  What a round waits for are the two warp-wide maxima and the winner's next number, which is there
-// already.  The kernel is all latency, of its instructions too, which every launch fetches anew: it is kept short.  One request of four beams: 6,500 cycles,
-// of which loads and normalisers 2,000, merging 1,800, ranking 1,100.
+// already.  The kernel is all latency.  One request of four beams: 6,500 cycles, of which loads and normalisers 2,000, merging 1,800, ranking 1,100.
 __global__ void __launch_bounds__(1024) beam_join_kernel(const u64* __restrict__ best, const float2* __restrict__ sums, int parts, int K, int V, int rows,
                                                          int beams, int end_token, bool rounds, const float* scores, int* tokens, int* parents,
                                                          float* out_scores, float* ended) {
