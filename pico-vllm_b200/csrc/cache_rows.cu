@@ -4,6 +4,7 @@
 // A tensor is [outer, rows, ...] with the bytes of a row in one piece; "row r" is the rows r of all its outer entries (a page of every layer, the
 // state of a request in every layer).  Sizes, strides and starts may be any: 16 bytes go at a time where all of them allow it.
 #include "common.cuh"
+#include <atomic>
 
 #define ROWS_TENSORS 16                                         // tensors of one launch
 #define ROWS_THREADS 256
@@ -13,12 +14,27 @@
 #define SHIFT_SPAN (ROWS_THREADS * SHIFT_LOADS)
 #define ROWS_BEAMS 32                                           // places of a group: lanes of a warp
 
-__device__ int g_rows_status = 0;    // 0 = fine; 1 = an index outside a tensor was passed over
-// Reads the word and sets it back.
+__device__ unsigned g_rows_missed = 0;  // how often an index outside a tensor was met (and passed over); only ever counted up
+// *out: has one been met since this was asked last, on this device?  Waits for the device first: the calls may be on any stream, and a copy from here waits for
+// none of those that PyTorch makes.  What was told last is kept on the host, so that nothing that a kernel counts meanwhile is wiped.
 PICO_API int pico_rows_status(int* out) {
-    const cudaError_t e = cudaMemcpyFromSymbol(out, g_rows_status, sizeof(int), 0, cudaMemcpyDeviceToHost);
-    const int fine = 0;
-    return (int)(e == cudaSuccess && *out ? cudaMemcpyToSymbol(g_rows_status, &fine, sizeof(int), 0, cudaMemcpyHostToDevice) : e);
+    static std::atomic<unsigned> told[64];
+    int dev = 0;
+    unsigned now = 0;
+    *out = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 64)) return PICO_ERR_SIZE;
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&now, g_rows_missed, sizeof(now), 0, cudaMemcpyDeviceToHost);
+    if (e != cudaSuccess) return (int)e;
+    // (two threads that ask at once: one of them tells, and an older count never takes the place of a newer)
+    unsigned before = told[dev].load();
+    while ((int)(now - before) > 0)
+        if (told[dev].compare_exchange_weak(before, now)) {
+            *out = 1;
+            break;
+        }
+    return 0;
 }
 
 struct RowTensor {
@@ -131,7 +147,8 @@ __global__ void __launch_bounds__(ROWS_THREADS) copy_rows_kernel(RowTensors ts, 
     const int s = src[blockIdx.y], d = dst[blockIdx.y];
     if (s < 0 || d < 0 || s == d) return;
     if (s >= t.rows || d >= t.rows) {
-        if (threadIdx.x == 0) g_rows_status = 1;
+        // (one block of the tensor counts)
+        if (threadIdx.x == 0 && blockIdx.x == t.first) atomicAdd(&g_rows_missed, 1u);
         return;
     }
     if (SHIFTED) copy_shifted(t, blockIdx.x - t.first, s, d);
@@ -183,7 +200,7 @@ __global__ void __launch_bounds__(ROWS_THREADS) reorder_rows_kernel(RowTensors t
         int from = __shfl_sync(0xffffffffu, slot, parent & 31);
         bool wanted = p < places && parent != p;
         if (wanted && (parent < 0 || parent >= places || slot < 0 || slot >= ts.rows || from < 0 || from >= ts.rows)) {
-            g_rows_status = 1;
+            if (blockIdx.x == 0) atomicAdd(&g_rows_missed, 1u);          // (one block of the group counts)
             wanted = false;
         }
         // the places that wait to take over what place p holds

@@ -409,8 +409,8 @@ def check_kernel_status() -> None:
     """Raises KernelError when a kernel gave up a bounded wait (on a TMA copy or a tensor-core barrier)
     since the library was loaded: such a block leaves its part of the result unwritten, so the
     tokens computed since are not to be trusted; also when copy_pages or reorder_states met an index
-    outside a tensor.  Reads four status words from the device (a few synchronous 4-byte copies), five
-    once rows of a cache have been moved; does nothing before the library was first used."""
+    outside a tensor, on whatever stream.  Reads four status words from the device (a few synchronous 4-byte copies); once rows of a
+    cache have been moved it also waits for the device and reads a fifth.  Does nothing before the library was first used."""
     if _lib is None:
         return
     bad = [name for name, word in (("paged_decode_tma (decode attention)", tma_status()),
@@ -1105,9 +1105,10 @@ _rows_used = False
 
 
 def rows_status() -> int:
-    """0, or 1 when copy_pages or reorder_states met an index outside a tensor (and passed it over) since this was asked last."""
+    """0, or 1 when copy_pages or reorder_states met an index outside a tensor (and passed it over) on the current device since this was asked last.
+    Waits for everything that was launched on the device, on whatever stream."""
     out = ctypes.c_int(0)
-    library().pico_rows_status(ctypes.addressof(out))
+    _check(library().pico_rows_status(ctypes.addressof(out)), "rows_status")
     return out.value
 
 
