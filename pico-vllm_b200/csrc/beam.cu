@@ -439,8 +439,11 @@ PICO_API int pico_beam_select(const float* logits, long long row_stride, int gro
     const int n = rows * parts * K;
     const size_t smem = (size_t)(n + rows * ((parts + 1) / 2) * K) * sizeof(u64) + (size_t)rows * K * sizeof(int);
     if (smem > 40 * 1024) {             // beside the kernel's own
-        const cudaError_t e = cudaFuncSetAttribute(beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return (int)cudaGetLastError();
+        const cudaError_t e = pico_allow_smem<beam_join_kernel>(smem);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return (int)e;
+        }
     }
     // a round takes some 100 cycles or more, as many warps as there are rows share the multiprocessor; a level of merging 350, or two a number (16 rows of 8
     // beams in 19 parts: by rounds 10.7 us, by levels 11.8; two of 28 beams in 16 parts 17.6 and 14.1)

@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 #include <math.h>
+#include <mutex>
 
 #define PICO_API extern "C" __attribute__((visibility("default")))
 
@@ -105,6 +106,23 @@ static inline int pico_num_sms() {
         cached[dev] = sms;
     }
     return cached[dev];
+}
+
+// Lets launches of a kernel on the current device take up to so many bytes of dynamic shared memory.  The limit belongs to the kernel, and
+// host threads that launch it share it: it is raised where it is too low and never lowered, so that no thread takes it away from a launch of another one.
+template <auto Kernel>
+static cudaError_t pico_allow_smem(size_t bytes) {
+    static std::mutex one_at_a_time;
+    static size_t allowed[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> guard(one_at_a_time);
+    if (bytes <= allowed[dev]) return cudaSuccess;
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) allowed[dev] = bytes;
+    return e;
 }
 
 // Programmatic dependent launch: every kernel of this library is launched with the attribute that
