@@ -354,7 +354,7 @@ static void tile_launch(const T* q, const T* k, const T* v, T* out, TileArgs a, 
     const size_t ring = (size_t)(RT == 32 ? 1 : 4) * 2 * KT * ld * sizeof(float);
     const size_t merge = (size_t)(RT == 32 ? 1 : 4) * RT * (ld + 2) * sizeof(float);
     const size_t smem = fixed + (ring > merge ? ring : merge);
-    cudaFuncSetAttribute(paged_attention_tiled_kernel<T, NJ, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    pico_allow_smem<paged_attention_tiled_kernel<T, NJ, RT>>(smem);
     const bool side = tile_side_by_side(RT, a.part_keys);
     pico_launch((paged_attention_tiled_kernel<T, NJ, RT>), dim3((unsigned)a.T * a.row_chunks * (side ? a.n_splits : 1), a.nkv, side ? 1 : a.n_splits), dim3(128), smem, stream, q, k, v,
                 out, a);

@@ -475,7 +475,7 @@ PICO_API int pico_paged_prefill_mma(const void* q, int q_row_stride, const void*
     const float cap_log2 = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, cap_2x = softcap > 0.f ? 2.0f * scale / softcap : 0.f;
 #define LAUNCH_PREFILL_X(HD, X)                                                                                     \
     do {                                                                                                            \
-        cudaFuncSetAttribute(paged_prefill_mma_kernel<HD, X>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
+        pico_allow_smem<paged_prefill_mma_kernel<HD, X>>(smem);                                                     \
         pico_launch((paged_prefill_mma_kernel<HD, X>), dim3(grid), dim3(MMA_THREADS), smem, stream,                 \
             (const bf16*)q, q_row_stride, (const bf16*)k_pages, (const bf16*)v_pages, (bf16*)out, seg_list, cu_q,   \
             positions, block_table, table_stride, nh, nkv, hd, page_size, window, scale_log2, cap_log2, cap_2x,     \
@@ -513,7 +513,7 @@ PICO_API int pico_paged_decode_mma(const void* q, int q_row_stride, const void* 
     const float cap_log2 = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f, cap_2x = softcap > 0.f ? 2.0f * scale / softcap : 0.f;
 #define LAUNCH_DECODE_X(HD, X)                                                                                     \
     do {                                                                                                           \
-        cudaFuncSetAttribute(paged_decode_mma_kernel<HD, X>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
+        pico_allow_smem<paged_decode_mma_kernel<HD, X>>(smem);                                                     \
         pico_launch((paged_decode_mma_kernel<HD, X>), dim3(grid), dim3(MMA_THREADS), smem, stream,                 \
             (const bf16*)q, q_row_stride, (const bf16*)k_pages, (const bf16*)v_pages, (bf16*)out, part_o, part_ml, \
             tok_list, tok_seg, positions, block_table, table_stride, nh, nkv, hd, page_size, window, scale_log2,   \

@@ -778,7 +778,7 @@ PICO_API int pico_paged_prefill_tcgen05(const void* k_map, const void* v_map, co
     memcpy(&vm, v_map, sizeof(CUtensorMap));
 #define LAUNCH_TCA(HD, CAP, EXTRA)                                                                                              \
     do {                                                                                                                 \
-        cudaFuncSetAttribute(paged_prefill_tcgen05_kernel<HD, CAP, EXTRA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
+        pico_allow_smem<paged_prefill_tcgen05_kernel<HD, CAP, EXTRA>>(smem);                                             \
         pico_launch((paged_prefill_tcgen05_kernel<HD, CAP, EXTRA>), grid, dim3(TCA_THREADS), smem, stream, km, vm, (const bf16*)q, \
                     q_row_stride, (bf16*)out, seg_list, cu_q, positions, block_table, table_stride, nh, nkv, page_size,  \
                     window, scale_log2, cap_log2, cap_2x, part_o, part_ml, counters, n_rows, n_parts, split_min, slopes, chunk, sinks, rates); \

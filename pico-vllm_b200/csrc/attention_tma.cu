@@ -524,7 +524,7 @@ static bool tma_cluster_query(int size, size_t smem) {
         cudaGetLastError();
         return false;
     }
-    cudaFuncSetAttribute(paged_decode_tma_kernel<HD, ST, CW, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    pico_allow_smem<paged_decode_tma_kernel<HD, ST, CW, NT, MODE>>(smem);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(size, 1, 1);
     cfg.blockDim = dim3((CW + 1) * 32);
@@ -596,8 +596,7 @@ PICO_API int pico_paged_decode_tma(const void* k_map, const void* v_map, const v
     if (n_splits > 1 && !cluster && (!part_o || !part_ml)) return PICO_ERR_SIZE;
 #define LAUNCH_TMA_C(HD, NT, MODE)                                                                                      \
     do {                                                                                                                \
-        cudaFuncSetAttribute(paged_decode_tma_kernel<HD, TMA_STAGES_MANY, 4, NT, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                             (int)smem);                                                                                \
+        pico_allow_smem<paged_decode_tma_kernel<HD, TMA_STAGES_MANY, 4, NT, MODE>>(smem);                               \
         pico_launch_cluster((paged_decode_tma_kernel<HD, TMA_STAGES_MANY, 4, NT, MODE>), grid, dim3(5 * 32), smem, stream, \
                             cluster ? n_splits : 1, km, vm, (const bf16*)q, q_row_stride, (bf16*)out, part_o,           \
                             part_ml, tok_list, tok_seg, positions, block_table, table_stride, nh, nkv, page_size,       \

@@ -1180,16 +1180,17 @@ PICO_API int pico_gated_delta_chunks(const float* prep, const float* v, int v_st
                          (blocks + three - 1) / three < (blocks + two - 1) / two;
     const size_t sm1 = (size_t)(crowded ? shared : other + q_floats + v_floats) * sizeof(float);
     auto prepare = crowded ? delta_chunk_prepare_kernel<true> : delta_chunk_prepare_kernel<false>;
-    cudaFuncSetAttribute(prepare, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm1);
+    if (crowded) pico_allow_smem<delta_chunk_prepare_kernel<true>>(sm1);
+    else pico_allow_smem<delta_chunk_prepare_kernel<false>>(sm1);
     pico_launch(prepare, dim3(chunks, G), dim3(256), sm1, stream, prep, P, v, v_stride, cu_q, positions, S, coef, u, H, G, d, dv, keep_v);
     const dim3 grid((dv + DC_NC - 1) / DC_NC, H, S);
     size_t sm2 = (size_t)(2 * (DC_C * DC_LDT + DC_C * DC_LDM + 2 * DC_C + DC_C * DC_LDU) + DC_WARPS * 512 + DC_C * 32) * sizeof(float);
     // (one block a multiprocessor where there are enough of them: see pico_gated_delta_rule)
     if ((long long)grid.x * grid.y * grid.z <= pico_num_sms() && sm2 < 116 * 1024) sm2 = 116 * 1024;
-    cudaFuncSetAttribute(delta_chunk_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm2);
+    pico_allow_smem<delta_chunk_kernel>(sm2);
     pico_launch(delta_chunk_kernel, grid, dim3(32 * (DC_WARPS + 4)), sm2, stream, prep, P, state, seg_slots, cu_q, positions, (const float*)coef, u, s0, H, G, d, dv);
     const size_t sm3 = (size_t)(DC_OC * DC_LD + DC_C * DC_LD + DC_C * DC_OC + DC_C * DC_C + DC_C) * sizeof(float);
-    cudaFuncSetAttribute(delta_chunk_out_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm3);
+    pico_allow_smem<delta_chunk_out_kernel>(sm3);
     pico_launch(delta_chunk_out_kernel, dim3(chunks, H, (dv + DC_OC - 1) / DC_OC), dim3(128), sm3, stream, prep, P, cu_q, positions, S,
                 (const float*)coef, (const float*)u, (const float*)s0, out, out_stride, H, G, d, dv);
     return pico_launch_status();
@@ -1213,7 +1214,7 @@ PICO_API int pico_gated_delta_rule(const float* prep, const float* v, int v_stri
         size_t smem = (size_t)2 * DR_TOK * ((PH ? 2 : 3) * N * L + 16 + 4) * sizeof(float);                                 \
         if (alone && smem < 116 * 1024) smem = 116 * 1024;                                                                  \
         if (smem > 48 * 1024)                                                                                               \
-            cudaFuncSetAttribute(gated_delta_rule_kernel<N, L, PH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);  \
+            pico_allow_smem<gated_delta_rule_kernel<N, L, PH>>(smem);                                                       \
         pico_launch((gated_delta_rule_kernel<N, L, PH>), grid, dim3(16 * L), smem, stream, prep, P, v, v_stride, state,     \
                     seg_slots, cu_q, positions, out, out_stride, H, G, d, dv);                                              \
     } while (0)
@@ -1227,7 +1228,7 @@ PICO_API int pico_gated_delta_rule(const float* prep, const float* v, int v_stri
         size_t smem = (size_t)(2 * DB_TOK * (2 * N * L + 16 + 12) + DB_TOK / 4 * DB_COEF) * sizeof(float);                  \
         if (alone && smem < 116 * 1024) smem = 116 * 1024;                                                                  \
         if (smem > 48 * 1024)                                                                                               \
-            cudaFuncSetAttribute(gated_delta_block_kernel<N, L, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
+            pico_allow_smem<gated_delta_block_kernel<N, L, C>>(smem);                                                       \
         pico_launch((gated_delta_block_kernel<N, L, C>), grid, dim3(16 * L / C), smem, stream, prep, P, v, v_stride, state, \
                     seg_slots, cu_q, positions, out, out_stride, H, G, d, dv, vec, below > 0 ? below : 0x7fffffff);                                         \
     } while (0)

@@ -124,7 +124,7 @@ PICO_API int pico_add_rmsnorm(float* x, const void* delta, const float* weight, 
 #define LAUNCH_NORM(TA, V4)                                                                                          \
     do {                                                                                                             \
         if (smem > 48 * 1024)                                                                                        \
-            cudaFuncSetAttribute(add_rmsnorm_kernel<TA, V4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
+            pico_allow_smem<add_rmsnorm_kernel<TA, V4>>(smem);                                                       \
         pico_launch((add_rmsnorm_kernel<TA, V4>), dim3(R), dim3(threads), smem, stream, x, (const TA*)delta, weight,  \
                     (TA*)out, rows, H, eps);                                                                         \
     } while (0)

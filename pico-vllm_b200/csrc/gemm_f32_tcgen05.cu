@@ -367,7 +367,7 @@ PICO_API int pico_gemm_f32(const float* x, long long ldx, const float* w, float*
     rc = tf_map(&wm, w, N, K, K, TF_BM);
     if (rc) return rc;
     const size_t smem = (size_t)TF_STAGES * TF_RAW + (size_t)TF_SPLITS * 3 * TF_PART + 1024;
-    cudaFuncSetAttribute(gemm_f32_tcgen05_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    pico_allow_smem<gemm_f32_tcgen05_kernel>(smem);
     pico_launch(gemm_f32_tcgen05_kernel, dim3((N + TF_BM - 1) / TF_BM, (M + a.m_tile - 1) / a.m_tile, a.parts), dim3(TF_THREADS), smem, stream, xm, wm, a);
     if (a.parts > 1) pico_launch(gemm_f32_sum_kernel, dim3((unsigned)(((size_t)M * N / 4 + 255) / 256)), dim3(256), 0, stream, (const float*)scratch, out, a);
     return pico_launch_status();

@@ -541,7 +541,7 @@ static int tp_launch(const void* x, int ldx, const void* w, const TpArgs& a, cud
     rc = tp_make_map(&wm, w, GROUPED ? (long long)a.E * a.N : a.N, a.K, a.K, BN / 2);
     if (rc) return rc;
     const size_t smem = (size_t)STAGES * STAGE_BYTES + (2 * STAGES + 4) * 8 + 16 + 1024 + (GROUPED ? 3 * (a.E + 1) * sizeof(int) : 0);
-    cudaFuncSetAttribute(gemm_tcgen05_pair_kernel<BN, EPI, STAGES, MB, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    pico_allow_smem<gemm_tcgen05_pair_kernel<BN, EPI, STAGES, MB, GROUPED>>(smem);
     const int n_out = tp_is_glu(EPI) ? a.N / 2 : a.N;
     const int cols = tp_is_glu(EPI) ? BN / 2 : BN;
     // (the groups' tiles: at most so many; the kernel reads how many there are)
@@ -923,7 +923,7 @@ static int tg_launch(const void* x, const void* w, const TgArgs& a, cudaStream_t
     rc = GLU && !a.sixteens ? tg_make_glu_map(&wm, w, a) : tp_make_map(&wm, w, (long long)a.E * a.N, a.K, a.K, GLU ? 16 : TP_BM);
     if (rc) return rc;
     const size_t smem = TG_RING + (2 * TG_STAGES + 2) * 8 + 8 + 8 * sizeof(float) + (2 * (a.E + 1) + 1) * sizeof(int) + 1024;
-    cudaFuncSetAttribute(gemm_tcgen05_group_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    pico_allow_smem<gemm_tcgen05_group_kernel<EPI>>(smem);
     const int n_out = GLU ? a.N / 2 : a.N, n_tiles = (n_out + (GLU ? 128 : 256) - 1) / (GLU ? 128 : 256);
     const long long most = ((long long)a.n / 64 + (a.E < a.n ? a.E : a.n)) * n_tiles;      // (the kernel reads how many tiles there are)
     const int max_pairs = tp_num_sms() / 2, pairs = most < max_pairs ? (int)most : max_pairs;

@@ -152,7 +152,7 @@ PICO_API int pico_hyper_step(float* x, const void* y, const float* mix, const fl
 #define HC_LAUNCH_V(TA, V)                                                                                              \
     do {                                                                                                                \
         if (smem > 48 * 1024)                                                                                           \
-            cudaFuncSetAttribute(hyper_step_kernel<TA, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);     \
+            pico_allow_smem<hyper_step_kernel<TA, V>>(smem);                                                            \
         pico_launch((hyper_step_kernel<TA, V>), dim3(R), dim3(256), smem, stream, x, (const TA*)y, mix, outw, inw, norm_w, eps, \
                     (TA*)h, rows, sum_out, S, D);                                                                       \
     } while (0)

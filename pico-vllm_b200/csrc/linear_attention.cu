@@ -287,8 +287,7 @@ PICO_API int pico_decay_linear_attention(const void* proj, int row_stride, int q
 #define LA_LAUNCH(TA, DPL, SO, EX)                                                                                       \
     do {                                                                                                                 \
         if (smem > 48 * 1024)                                                                                            \
-            cudaFuncSetAttribute(decay_linear_attention_kernel<TA, DPL, SO, EX>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                                 (int)smem);                                                                             \
+            pico_allow_smem<decay_linear_attention_kernel<TA, DPL, SO, EX>>(smem);                                       \
         pico_launch((decay_linear_attention_kernel<TA, DPL, SO, EX>), grid, dim3(LA_WARPS * 32), smem, stream,           \
                     (const TA*)proj, row_stride, q_off, k_off, v_off, decay, state, seg_slots, cu_q, positions, out, H, d, \
                     dv, act, chunk, max_chunks, chunk_state);                                                            \

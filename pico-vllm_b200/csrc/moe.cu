@@ -466,7 +466,7 @@ PICO_API int pico_moe_route(const void* h, const float* wr, const float* br, int
 #define LAUNCH_ROUTE(TA, TOK, VEC)                                                                                        \
     do {                                                                                                                  \
         if (smem > 48 * 1024)                                                                                             \
-            cudaFuncSetAttribute(moe_route_kernel<TA, TOK, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
+            pico_allow_smem<moe_route_kernel<TA, TOK, VEC>>(smem);                                                        \
         pico_launch((moe_route_kernel<TA, TOK, VEC>), grid, dim3(256), smem, stream, (const TA*)h, wr, br, T, D, E, top, mode, idx, wgt, choice_bias, weight_scale, groups, groups_keep, renorm); \
     } while (0)
     const bool vec = D % (dtype == PICO_F32 ? 4 : 8) == 0 && ((uintptr_t)h & 15) == 0;

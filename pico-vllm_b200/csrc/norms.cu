@@ -332,7 +332,7 @@ PICO_API int pico_post_add_norm(float* x, const void* delta, const float* post_w
 #define LAUNCH_PAN(TA, V4)                                                                                                \
     do {                                                                                                                  \
         if (smem > 48 * 1024)                                                                                             \
-            cudaFuncSetAttribute(post_add_norm_kernel<TA, V4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);   \
+            pico_allow_smem<post_add_norm_kernel<TA, V4>>(smem);                                                          \
         pico_launch((post_add_norm_kernel<TA, V4>), dim3(R), dim3(threads), smem, stream, x, (const TA*)delta, post_w,    \
                     post_kind, post_eps, w, kind, eps, (TA*)out, rows, H, post_groups, groups);                           \
     } while (0)

@@ -294,8 +294,7 @@ PICO_API int pico_gated_linear_attention(const float* q, int q_stride, const flo
 #define GL_LAUNCH(DPL, G, SO, XC)                                                                                        \
     do {                                                                                                                 \
         if (smem > 48 * 1024)                                                                                            \
-            cudaFuncSetAttribute(gated_linear_attention_kernel<DPL, G, SO, XC>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                                 (int)smem);                                                                             \
+            pico_allow_smem<gated_linear_attention_kernel<DPL, G, SO, XC>>(smem);                                        \
         pico_launch((gated_linear_attention_kernel<DPL, G, SO, XC>), grid, dim3(GL_WARPS * 32), smem, stream, q, q_stride, k, \
                     k_stride, v, v_stride, gate, gate_stride, state, seg_slots, cu_q, positions, out, out_stride, H, qk_rep, d, dv,   \
                     chunk, max_chunks, chunk_state, chunk_gate);                                                         \

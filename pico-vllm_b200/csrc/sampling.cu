@@ -363,7 +363,7 @@ static size_t sample_bytes(int per) { return 2 * SAMPLE_BINS * sizeof(u64) + (si
 template <bool KEEP>
 static bool sample_sixteen(size_t smem) {
     if (cudaFuncSetAttribute(sample_row_kernel<KEEP, 16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-        cudaFuncSetAttribute(sample_row_kernel<KEEP, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+        pico_allow_smem<sample_row_kernel<KEEP, 16>>(smem) != cudaSuccess) {
         cudaGetLastError();
         return false;
     }
@@ -416,7 +416,7 @@ PICO_API int pico_sample(const float* logits, int row_stride, int R, int V, cons
         const float *t = temperature ? temperature + r0 : nullptr, *tp = top_p ? top_p + r0 : nullptr, *u = uniform ? uniform + r0 : nullptr;
 #define SAMPLE_LAUNCH(K, B)                                                                                                      \
     do {                                                                                                                         \
-        cudaFuncSetAttribute(sample_row_kernel<K, B>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                   \
+        pico_allow_smem<sample_row_kernel<K, B>>(smem);                                                                          \
         pico_launch_cluster((sample_row_kernel<K, B>), dim3(B, rows), dim3(SAMPLE_THREADS), smem, stream, B, lg, row_stride, V, t, tp, u, \
                             out + r0, per, vec);                                                                                 \
     } while (0)

@@ -496,7 +496,7 @@ static void sg_launch_one(const SkinnyArgs& a, int tiles, int grid, cudaStream_t
     const size_t smem = (size_t)SG_WARPS * STAGES * (XPRE ? 16 : 16 + MT * 8) * SG_LD * sizeof(bf16) +
                         (XPRE ? (size_t)MT * 8 * x_ld * sizeof(bf16) : 0) + (size_t)SG_WARPS * 16 * MT * 8 * sizeof(float) +
                         (EPI == SG_ARGMAX ? (size_t)2 * MT * 8 * sizeof(float) : 0);
-    cudaFuncSetAttribute(skinny_gemm_kernel<MT, EPI, STAGES, XPRE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    pico_allow_smem<skinny_gemm_kernel<MT, EPI, STAGES, XPRE>>(smem);
     pico_launch((skinny_gemm_kernel<MT, EPI, STAGES, XPRE>), dim3(grid), dim3(SG_THREADS), smem, stream, a, tiles, x_ld);
 }
 

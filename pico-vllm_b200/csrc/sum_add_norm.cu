@@ -85,7 +85,7 @@ PICO_API int pico_sum_add_norm(float* x, const void* d0, const float* w0, int k0
 #define SAN_LAUNCH(TA)                                                                                                     \
     do {                                                                                                                   \
         if (smem > 48 * 1024)                                                                                              \
-            cudaFuncSetAttribute(sum_add_norm_kernel<TA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);         \
+            pico_allow_smem<sum_add_norm_kernel<TA>>(smem);                                                                \
         pico_launch((sum_add_norm_kernel<TA>), dim3(R), dim3(threads), smem, stream, x, a, b, c, w, kind, eps, (TA*)out, rows, H); \
     } while (0)
     if (act_dtype == PICO_F32) SAN_LAUNCH(float);

@@ -45,3 +45,29 @@ def test_choices_of_different_sizes():
                 torch.cuda.current_stream().synchronize()
                 assert all(torch.equal(a, b) for a, b in zip(got, want[k]))
     together([lambda: job(0), lambda: job(1), lambda: job(0)])
+
+
+def test_router_and_norms_of_different_widths():
+    """Kernels whose rows lie in shared memory take more of it for wider rows."""
+    from pico_vllm_b200 import ops
+    g = torch.Generator().manual_seed(8)
+
+    def routing(width):
+        h, w = torch.randn(6, width, generator=g).to(DEV), (torch.randn(64, width, generator=g) / width ** 0.5).to(DEV)
+        return lambda: ops.moe_route(h, w, None, 4)
+
+    def norm(width):
+        x, w = torch.randn(5, width, generator=g).to(DEV), torch.randn(width, generator=g).to(DEV)
+        return lambda: (ops.add_rmsnorm(x, None, w, 1e-6, torch.empty_like(x)),)
+    calls = [make(width) for make in (routing, norm) for width in (14000, 20000)]
+    want = [[t.clone() for t in c()] for c in calls]
+    torch.cuda.synchronize()
+
+    def job(k):
+        for i in range(2000):
+            for c in (k, 2 + k):
+                r = calls[c]()
+                if i % 500 == 0:
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(r, want[c]))
+    together([lambda: job(0), lambda: job(1), lambda: job(0)])
