@@ -5,6 +5,7 @@
 from torch's global generator and always stops at the tokenizer's end token."""
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -34,8 +35,8 @@ class SamplingParams:
 @dataclass
 class BeamParams:
     """Options of beam search: the ``beams`` best continuations are kept at every token.  A hypothesis is worth the sum of its tokens'
-    log-probabilities divided by its length to the power ``length_penalty`` (its end token counted; 0: the sum itself).  The
-    reference has no beam search."""
+    log-probabilities divided by its length to the power ``length_penalty`` (its end token counted; 0: the sum itself;
+    max_new_tokens ** length_penalty is at most 2 ** 873).  The reference has no beam search."""
     beams: int = 4
     max_new_tokens: int = 16
     length_penalty: float = 1.0
@@ -49,6 +50,11 @@ class BeamParams:
             raise ConfigError("max_new_tokens must be at least 1")
         if not 0 <= self.length_penalty < float("inf"):
             raise ConfigError("length_penalty must be a number >= 0")
+        # the value of a hypothesis is to be a number of full precision: a sum of log-probabilities as small as a float32 holds (2^-149), divided, is
+        # not below the smallest such float64 (2^-1022)
+        if self.max_new_tokens > 1 and self.length_penalty > 873 / math.log2(self.max_new_tokens):
+            raise ConfigError(f"length_penalty {self.length_penalty} with max_new_tokens {self.max_new_tokens}: a length to that power is beyond the "
+                              f"numbers that hypotheses can be ranked by (at most {873 / math.log2(self.max_new_tokens):.1f})")
         if self.num_return is None:
             self.num_return = self.beams
         if not 1 <= self.num_return <= self.beams:
