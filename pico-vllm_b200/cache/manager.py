@@ -197,7 +197,7 @@ class CacheManager:
     def reorder(self, slots: Sequence[Sequence[int]], parents: Sequence[Sequence[int]], on_device=None) -> None:
         """Passes on what requests of a family hold: slots[f][p] holds afterwards what slots[f][parents[f][p]] held, all at once, for every
         family f.  The members of a family hold equally many tokens.  ``on_device``: (slots, parents) as int32 tensors, if
-        the caller has them there (the states are moved by them).  Needs no free page."""
+        the caller has them there (the states are moved by them).  Needs no free page.  Where there are states, a family has 32 members at most."""
         flat = [s for line in slots for s in line]
         if len(set(flat)) != len(flat) or len(slots) != len(parents):
             raise PicoError("a slot belongs to one family, and every family has its parents")
@@ -211,6 +211,10 @@ class CacheManager:
         moved = [(line, family) for line, family in zip(slots, parents) if any(q != p for p, q in enumerate(family))]
         if not moved:
             return
+        if self.state_stacks:
+            from .. import ops
+            if max(len(line) for line, _ in moved) > ops.BEAM_MAX:      # (before anything moves)
+                raise PicoError(f"states are passed on within families of {ops.BEAM_MAX} at most")
         for g in self.groups:
             src: List[int] = []
             dst: List[int] = []
@@ -220,7 +224,6 @@ class CacheManager:
             self._give_back(g, gone)
             self._copy_rows(g.tensors.values(), src, dst)
         if self.state_stacks:
-            from .. import ops
             if on_device is None:
                 most = max(len(line) for line, _ in moved)
 
