@@ -266,7 +266,7 @@ __device__ __forceinline__ unsigned beam_winner(u64 v) {
 // costs a few dependent loads however long the lists are.  Then the first warp ranks the rows' lists against one another, a lane for each row,
 // until B candidates that go on are found.  What a round waits for are the two warp-wide maxima and the winner's next number, which is there
 // already.  The kernel is all latency.  One request of four beams: 6,500 cycles, of which loads and normalisers 2,000, merging 1,800, ranking 1,100.
-__global__ void __launch_bounds__(1024) beam_join_kernel(const u64* __restrict__ best, const float2* __restrict__ sums, int parts, int K, int V, int rows,
+__global__ void __launch_bounds__(1024) beam_join_kernel(const u64* __restrict__ best, const float2* __restrict__ sums, int parts, int K, int rows,
                                                          int beams, int end_token, bool rounds, const float* scores, int* tokens, int* parents,
                                                          float* out_scores, float* ended) {
     pdl_launch_dependents();
@@ -405,7 +405,8 @@ __global__ void __launch_bounds__(1024) beam_join_kernel(const u64* __restrict__
     if (lane < rows) ended[g * rows + lane] = end_k < 0 ? -INFINITY : (float)beam_unorder(list[end_k]);
 }
 
-#define BEAM_JOIN_KEYS 8192     // candidates that a block of beam_join_kernel has room for in shared memory (up to 136 KB)
+#define BEAM_JOIN_KEYS 8192     // candidates that a block of beam_join_kernel has room for in shared memory (with the merged ones and their tokens up to
+                                // 108 KB: 28 rows of 29 beams in 5 parts)
 
 // Parts of a row: as many as run at once over all rows (256 rows of 151,936 in 1 / 2 / 3 / 4 / 7 parts: 44 / 43 / 35 / 42 / 36 us with the join of then, now 32 in 3;
 // four rows in 7 / 10 / 19: 8.9 / 8.3 / 7.6), none shorter than a tile, and no more than the join (a lane each) and the scratch have room for.
@@ -456,7 +457,7 @@ PICO_API int pico_beam_select(const float* logits, long long row_stride, int gro
     pico_launch(vec ? beam_rows_kernel<true> : beam_rows_kernel<false>, dim3(parts, R), dim3(BEAM_THREADS), 0, stream, logits, row_stride, V, K, sets, per, best, sums);
     const int status = pico_launch_status();
     if (status) return status;
-    pico_launch(beam_join_kernel, dim3(groups), dim3(threads), smem, stream, (const u64*)best, (const float2*)sums, parts, K, V, rows, beams, end_token,
+    pico_launch(beam_join_kernel, dim3(groups), dim3(threads), smem, stream, (const u64*)best, (const float2*)sums, parts, K, rows, beams, end_token,
                 rounds, scores, tokens, parents, out_scores, ended);
     return pico_launch_status();
 }

@@ -17,7 +17,7 @@ from typing import Deque, List, Optional, Sequence, Tuple
 import torch
 
 from .. import ops
-from ..errors import ConfigError, OutOfPages, ScheduleError
+from ..errors import ConfigError, ScheduleError
 from ..sampling import BeamParams
 from .runner import StepItem
 

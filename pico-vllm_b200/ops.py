@@ -1003,6 +1003,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, end_toke
     child of beam p has place p, so that its cache can stay where it is; the others take the places that are left, in their order.
     A place for which there is no candidate has token -1, itself as parent and the score -infinity.
     ended float32 [G, rows]: v of (b, end_token) where that is among the best ``beams`` candidates of all, else -infinity.
+    (Values are ranked in 64 bits and rounded once at the end: a candidate whose v lies below float32's numbers is chosen like any other and has -infinity.)
 
     All four are views of one int32 buffer (floats by their bits; in that order), which ``out`` may give: contiguous int32
     [G * (3 * beams + rows)].  ``scores`` may be the new_scores of an earlier call with the same ``out``."""
