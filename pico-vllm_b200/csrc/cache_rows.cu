@@ -15,17 +15,21 @@
 #define ROWS_BEAMS 32                                           // places of a group: lanes of a warp
 
 __device__ unsigned g_rows_missed = 0;  // how often an index outside a tensor was met (and passed over); only ever counted up
-// *out: has one been met since this was asked last, on this device?  Waits for the device first: the calls may be on any stream, and a copy from here waits for
-// none of those that PyTorch makes.  What was told last is kept on the host, so that nothing that a kernel counts meanwhile is wiped.
-PICO_API int pico_rows_status(int* out) {
+// *out: has one been met since this was asked last, on this device, by what the stream has run?  Waits for the stream and for no other: waiting for the device would end
+// a recording that another thread is making.  What was told last is kept on the host and the count is never set back, so that nothing that a kernel counts
+// meanwhile, or on another stream, is lost: it is told the next time.  A stream that is being recorded is not asked.
+PICO_API int pico_rows_status(int* out, cudaStream_t stream) {
     static std::atomic<unsigned> told[64];
     int dev = 0;
     unsigned now = 0;
+    cudaStreamCaptureStatus recording = cudaStreamCaptureStatusNone;
     *out = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess && (dev < 0 || dev >= 64)) return PICO_ERR_SIZE;
-    if (e == cudaSuccess) e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&now, g_rows_missed, sizeof(now), 0, cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess) e = cudaStreamIsCapturing(stream, &recording);
+    if (e == cudaSuccess && recording != cudaStreamCaptureStatusNone) return 0;
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(&now, g_rows_missed, sizeof(now), 0, cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
     if (e != cudaSuccess) return (int)e;
     // (two threads that ask at once: one of them tells, and an older count never takes the place of a newer)
     unsigned before = told[dev].load();

@@ -90,7 +90,7 @@ def library():
         "pico_beam_select": [vp, i64, i32, i32, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp],
         "pico_copy_rows": [vp, i32, vp, vp, i32, vp],
         "pico_reorder_rows": [vp, i32, vp, vp, i32, i32, vp],
-        "pico_rows_status": [vp],
+        "pico_rows_status": [vp, vp],
         "pico_post_add_norm": [vp, vp, vp, i32, f32, vp, i32, f32, vp, vp, i32, i32, i32, i32, i32, vp],
         "pico_scale_softcap": [vp, i32, i32, i32, f32, f32, vp],
         "pico_latent_norm_store": [vp, i32, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, vp, f32, i32, i32, i32, i32, i32, vp, f32,
@@ -409,8 +409,9 @@ def check_kernel_status() -> None:
     """Raises KernelError when a kernel gave up a bounded wait (on a TMA copy or a tensor-core barrier)
     since the library was loaded: such a block leaves its part of the result unwritten, so the
     tokens computed since are not to be trusted; also when copy_pages or reorder_states met an index
-    outside a tensor, on whatever stream.  Reads four status words from the device (a few synchronous 4-byte copies); once rows of a
-    cache have been moved it also waits for the device and reads a fifth.  Does nothing before the library was first used."""
+    outside a tensor (calls on the current stream, which it waits for; those on other streams once they have run).  Reads four
+    status words from the device (a few synchronous 4-byte copies), five once rows of a cache have been moved; does nothing before
+    the library was first used."""
     if _lib is None:
         return
     bad = [name for name, word in (("paged_decode_tma (decode attention)", tma_status()),
@@ -1107,9 +1108,9 @@ _rows_used = False
 
 def rows_status() -> int:
     """0, or 1 when copy_pages or reorder_states met an index outside a tensor (and passed it over) on the current device since this was asked last.
-    Waits for everything that was launched on the device, on whatever stream."""
+    Waits for the current stream; what was called on another one is told here once it has run, and never lost."""
     out = ctypes.c_int(0)
-    _check(library().pico_rows_status(ctypes.addressof(out)), "rows_status")
+    _check(library().pico_rows_status(ctypes.addressof(out), _stream()), "rows_status")
     return out.value
 
 

@@ -1,7 +1,5 @@
 """Models whose next token hangs on the whole context, so that a beam that reads another one's keys, values or states goes another way: the small
 models of helpers.py with a head of their own (a tied, scaled table is mostly the last token's own row), and those with states."""
-import math
-
 import torch
 
 import beam_models
